@@ -86,7 +86,8 @@ int b200fc_set_sm_limit(int sms);
 int b200fc_set_decode_ctas_per_sm(int n);
 
 /* waits for `stream` and reports whether any kernel of this library gave up on a bounded wait since the last check
- * (B200FC_ERR_KERNEL); the _host entry points do this themselves */
+ * (B200FC_ERR_KERNEL), or met a page, row, length or position outside its range (B200FC_ERR_INVALID, see b200fc_paged_cache_t); the
+ * _host entry points do this themselves */
 int b200fc_sync_check(void* stream);
 /* Every wait inside a kernel (on a shared-memory barrier, on another GPU's arrival counter) is bounded; a wait that
  * runs out makes the kernel stop cleanly and b200fc_sync_check report B200FC_ERR_KERNEL.  Sets that bound for
@@ -282,6 +283,75 @@ typedef struct {
     float scale;
 } b200fc_attention_t;
 int b200fc_decode_attention(const b200fc_attention_t* a, void* stream);
+
+/* ---- paged key/value cache: appending to it, and attention over it (no reference counterpart) ----------------------- */
+/* A pool of pages of page_tokens tokens each, for Hkv kv heads of size D, and which of them the sequences of a call own.  Token t of sequence b
+ * lies in page page_table[b][t / page_tokens] at place t % page_tokens:
+ *     k + page * page_stride + head * head_stride + place * token_stride   (bytes; v has the same strides)
+ * dtype B200FC_BF16, or B200FC_S8 with one fp32 factor for each page and kv head, in k_scale and v_scale: cached value = int8 * factor.
+ * D: 64 or 128.  page_tokens: 16, 32, 64 or 128.  k, v and their strides 16-byte aligned, token_stride >= a token's D elements.
+ * Everything that page_table, seq_lens and row_start name is checked where it is read, on the device.  A sequence whose rows or length lie outside
+ * their buffers is left out (its rows of out are not written), a page outside [0, pages) is neither written nor read, and the next
+ * b200fc_sync_check on the device returns B200FC_ERR_INVALID once.  Table entries behind a sequence's last token may hold anything. */
+typedef struct {
+    int pages, page_tokens, Hkv, D, dtype;
+    void* k; void* v;
+    int64_t page_stride, head_stride, token_stride;
+    float* k_scale; float* v_scale;     /* B200FC_S8: factor of (page, head) at + page * scale_page_stride + head * 4 */
+    int64_t scale_page_stride;          /* bytes */
+    int B, max_pages;                   /* sequences, pages that a row of the table has room for */
+    const int32_t* page_table;          /* device [B, max_pages] */
+    int64_t table_stride;               /* bytes between its rows */
+    const int32_t* seq_lens;            /* device [B]: tokens of each sequence once the rows of the call are in the cache */
+} b200fc_paged_cache_t;
+
+/* Rows of the calls below: sequence b has rows [row_start[b], row_start[b + 1]) of the T rows (row_start: device [B + 1], rising), which are its
+ * LAST tokens: row r stands at place seq_lens[b] - (row_start[b + 1] - r).  row_start NULL: one row each, T = B.  A row at a negative place (more
+ * rows than tokens: a padded batch) belongs to no token.  Rows outside [row_start[0], row_start[B]) are left as they are. */
+
+/* Writes k and v of new rows into the cache, with the rotation of their positions applied to k, and rotates the rows of q as well.
+ *   rotation   (a, b) -> (a cos - b sin, b cos + a sin) for rot_dim / 2 pairs of components of each head: i with i + rot_dim / 2, or (interleaved)
+ *              2 i with 2 i + 1; the other components are kept.  cos and sin come from rot_cos, rot_sin [rot_positions, rot_dim / 2] fp32.  The position of a row
+ *              is its place in the sequence, or positions[r]; with axes = 3 (time, height, width), pairs [0, section[0]) take positions[0][r], the next
+ *              section[1] positions[1][r], and so on.  rot_dim 0: none.  A position outside the table rotates by nothing and is reported as above.
+ *   bf16       the fp32 results are rounded once.
+ *   int8       a page's factor is s = max(s of the tokens it holds already, largest new |value| / 127), new values are stored as rne(x / s), and where s
+ *              grew the older ones as rne(q * s_before / s), with fp32 products by 1 / s; a factor below 2^-126 is stored as 0.  A page of which the call
+ *              writes place 0 starts anew.  A page that holds or receives an infinity or a NaN has the factor NaN from then on.
+ * Two sequences of a call may share pages only where neither writes.  q NULL: none; q_out may be q itself (with q's strides), no other overlap.
+ * rot_dim: a multiple of 16, at most D.  q, k, v, q_out, rot_cos, rot_sin and their strides 16-byte aligned. */
+typedef struct {
+    const b200fc_paged_cache_t* cache;
+    int T;
+    const int32_t* row_start;
+    const void* k; int64_t k_row_stride, k_head_stride;          /* [T, Hkv, D] bf16; strides in bytes */
+    const void* v; int64_t v_row_stride, v_head_stride;
+    int H;                                                       /* query heads */
+    const void* q; int64_t q_row_stride, q_head_stride;          /* [T, H, D] bf16 */
+    void* q_out; int64_t q_out_row_stride, q_out_head_stride;
+    int rot_dim, interleaved, rot_positions;
+    const float* rot_cos; const float* rot_sin; int64_t rot_stride;   /* bytes between positions */
+    const int32_t* positions; int64_t position_stride;           /* device [axes, T] or NULL; bytes between axes */
+    int axes;                                                    /* 1 or 3 */
+    int section[3];                                              /* with axes = 3: pairs of each axis, rot_dim / 2 in all */
+} b200fc_kv_append_t;
+int b200fc_kv_append(const b200fc_kv_append_t* a, void* stream);
+
+/* out[r, h, :] = sum_j softmax_j(scale * q[r, h, :] . k_j) v_j over the cached tokens j of the row's sequence that are visible to its place p:
+ * j <= p, and with window > 0 only the last `window` of them (j > p - window) and the first `sinks` tokens of the sequence (j < sinks).  Rows that see no
+ * token are zeros.  Scores, softmax and sums are fp32; probabilities are rounded to bf16 for the product with v.  H / Hkv query heads share a kv head
+ * (any number).  max_rows: no sequence has more rows (a sequence that has is left out, as above).  q and out bf16, 16-byte aligned with their strides.
+ * What lies behind a sequence's last token, or is invisible to all its rows, may be anything, NaN included.  k and v of visible tokens: any bf16. */
+typedef struct {
+    const b200fc_paged_cache_t* cache;
+    int T, max_rows, H;
+    const int32_t* row_start;
+    const void* q; int64_t q_row_stride, q_head_stride;          /* [T, H, D] bf16 */
+    void* out; int64_t out_row_stride, out_head_stride;          /* [T, H, D] bf16 */
+    float scale;
+    int window, sinks;
+} b200fc_paged_attention_t;
+int b200fc_paged_attention(const b200fc_paged_attention_t* a, void* stream);
 
 /* ---- device memory for callers that do not link the CUDA runtime themselves ------------------------------------ */
 int b200fc_device_malloc(void** ptr, int64_t bytes);

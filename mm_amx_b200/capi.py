@@ -12,6 +12,7 @@ PACK_PLAIN, PACK_QUANT_TENSOR, PACK_INT8_CHANNEL, PACK_INT4_GROUP = 0, 1, 2, 3
 INT4_GROUP = 128
 
 c_int, c_i64, c_float, c_void_p = ctypes.c_int, ctypes.c_int64, ctypes.c_float, ctypes.c_void_p
+pointer = ctypes.pointer
 
 
 class Epilogue(ctypes.Structure):
@@ -35,6 +36,31 @@ class Attention(ctypes.Structure):
                 ("kv_batch_stride", c_i64), ("kv_head_stride", c_i64), ("kv_token_stride", c_i64), ("out", c_void_p),
                 ("out_batch_stride", c_i64), ("out_head_stride", c_i64), ("out_dtype", c_int), ("seq_lens", c_void_p),
                 ("scale", c_float)]
+
+
+class PagedCache(ctypes.Structure):
+    """b200fc_paged_cache_t"""
+    _fields_ = [("pages", c_int), ("page_tokens", c_int), ("Hkv", c_int), ("D", c_int), ("dtype", c_int), ("k", c_void_p), ("v", c_void_p),
+                ("page_stride", c_i64), ("head_stride", c_i64), ("token_stride", c_i64), ("k_scale", c_void_p), ("v_scale", c_void_p),
+                ("scale_page_stride", c_i64), ("B", c_int), ("max_pages", c_int), ("page_table", c_void_p), ("table_stride", c_i64),
+                ("seq_lens", c_void_p)]
+
+
+class KvAppend(ctypes.Structure):
+    """b200fc_kv_append_t; cache: pointer(PagedCache)"""
+    _fields_ = [("cache", ctypes.POINTER(PagedCache)), ("T", c_int), ("row_start", c_void_p), ("k", c_void_p), ("k_row_stride", c_i64),
+                ("k_head_stride", c_i64), ("v", c_void_p), ("v_row_stride", c_i64), ("v_head_stride", c_i64), ("H", c_int), ("q", c_void_p),
+                ("q_row_stride", c_i64), ("q_head_stride", c_i64), ("q_out", c_void_p), ("q_out_row_stride", c_i64),
+                ("q_out_head_stride", c_i64), ("rot_dim", c_int), ("interleaved", c_int), ("rot_positions", c_int), ("rot_cos", c_void_p),
+                ("rot_sin", c_void_p), ("rot_stride", c_i64), ("positions", c_void_p), ("position_stride", c_i64), ("axes", c_int),
+                ("section", c_int * 3)]
+
+
+class PagedAttention(ctypes.Structure):
+    """b200fc_paged_attention_t; cache: pointer(PagedCache)"""
+    _fields_ = [("cache", ctypes.POINTER(PagedCache)), ("T", c_int), ("max_rows", c_int), ("H", c_int), ("row_start", c_void_p),
+                ("q", c_void_p), ("q_row_stride", c_i64), ("q_head_stride", c_i64), ("out", c_void_p), ("out_row_stride", c_i64),
+                ("out_head_stride", c_i64), ("scale", c_float), ("window", c_int), ("sinks", c_int)]
 
 
 # name -> (restype, argtypes); every symbol include/b200fc.h declares
@@ -86,6 +112,8 @@ SIGNATURES = {
     "b200fc_mlp_decode_static_footprint": (c_i64, []),
     "b200fc_mlp_act": (c_void_p, [c_void_p]),
     "b200fc_decode_attention": (c_int, [ctypes.POINTER(Attention), c_void_p]),
+    "b200fc_kv_append": (c_int, [ctypes.POINTER(KvAppend), c_void_p]),
+    "b200fc_paged_attention": (c_int, [ctypes.POINTER(PagedAttention), c_void_p]),
     "b200fc_device_malloc": (c_int, [ctypes.POINTER(c_void_p), c_i64]),
     "b200fc_device_free": (c_int, [c_void_p]),
     "b200fc_memcpy": (c_int, [c_void_p, c_void_p, c_i64, c_void_p]),
@@ -305,6 +333,16 @@ def rmsnorm(x_ptr, ldx_bytes, M, K, eps, out_ptr, ldo_bytes, weight_ptr=None, st
 def decode_attention(desc, stream=None):
     """desc: capi.Attention; see b200fc_decode_attention in include/b200fc.h."""
     check(lib().b200fc_decode_attention(ctypes.byref(desc), stream))
+
+
+def kv_append(desc, stream=None):
+    """desc: capi.KvAppend; see b200fc_kv_append in include/b200fc.h."""
+    check(lib().b200fc_kv_append(ctypes.byref(desc), stream))
+
+
+def paged_attention(desc, stream=None):
+    """desc: capi.PagedAttention; see b200fc_paged_attention in include/b200fc.h."""
+    check(lib().b200fc_paged_attention(ctypes.byref(desc), stream))
 
 
 def add_round_bf16(a_ptr, b_ptr, out_ptr, n, stream=None):

@@ -58,6 +58,10 @@ int* kernel_status_word() {
 static int kernel_status_result(int v, int* p, cudaStream_t s) {
     if (v != 0) {
         cudaMemsetAsync(p, 0, sizeof(int), s);
+        if (v == kStatusPaged) {
+            set_error("paged cache: a page, row range, sequence length or position outside its range; what it names was left out");
+            return B200FC_ERR_INVALID;
+        }
         set_error("a kernel gave up on a bounded wait (code %d)", v);
         return B200FC_ERR_KERNEL;
     }
@@ -1205,6 +1209,16 @@ const void* b200fc_mlp_act(const b200fc_mlp_t* h) { return h ? h->m.act : nullpt
 int b200fc_decode_attention(const b200fc_attention_t* a, void* stream) {
     if (!a) { set_error("decode_attention: null descriptor"); return B200FC_ERR_INVALID; }
     return launch_decode_attention(*a, (cudaStream_t)stream);
+}
+
+int b200fc_kv_append(const b200fc_kv_append_t* a, void* stream) {
+    if (!a) { set_error("kv_append: null descriptor"); return B200FC_ERR_INVALID; }
+    return launch_kv_append(*a, (cudaStream_t)stream);
+}
+
+int b200fc_paged_attention(const b200fc_paged_attention_t* a, void* stream) {
+    if (!a) { set_error("paged_attention: null descriptor"); return B200FC_ERR_INVALID; }
+    return launch_paged_attention(*a, (cudaStream_t)stream);
 }
 
 int b200fc_device_malloc(void** ptr, int64_t bytes) {

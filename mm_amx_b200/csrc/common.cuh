@@ -101,6 +101,7 @@ void set_error(const char* fmt, ...);
 int cuda_fail(cudaError_t e, const char* what);
 void count_launch(int n = 1);
 int* kernel_status_word();  // device int, 0 = OK; kernels store a non-zero code when a bounded wait runs out
+constexpr int kStatusPaged = 16;   // what they store for a page, row, length or position outside its range (paged.cuh)
 int check_kernel_status(cudaStream_t s, int* pinned = nullptr);  // synchronises and reads it
 // growing device scratch owned by (device, stream, slot): work on one stream is ordered, so kernels launched on it
 // may share it; slot 0 = re-strided activations, slot 1 = split-K partial tiles of the GEMM and sums of folded parts of K, 3 = widened weight
@@ -252,6 +253,9 @@ int launch_gemm_tc_allreduce(const void* W_data, int W_K_pad, int W_N_pad, const
                              int N, const AllReduceDesc& ar, cudaStream_t s);
 // attention.cu
 int launch_decode_attention(const b200fc_attention_t& a, cudaStream_t s);
+// paged_append.cu, paged_attention.cu
+int launch_kv_append(const b200fc_kv_append_t& a, cudaStream_t s);
+int launch_paged_attention(const b200fc_paged_attention_t& a, cudaStream_t s);
 // matvec.cu
 int launch_matvec(const void* A, int dtype, int M, int K, int64_t lda, const void* b, void* c, cudaStream_t s);
 
