@@ -51,8 +51,13 @@ int launch_paged_attention(const b200fc_paged_attention_t& a, cudaStream_t s) {
     if ((long long)p.c.max_rows * p.G <= 16 && (long long)c.B * c.Hkv < (1LL << 31)) {
         DecParams d;
         d.a = p;
-        if (c.D == 128) return s8 ? launch_paged_decode_as<128, true>(d, s) : launch_paged_decode_as<128, false>(d, s);
-        return s8 ? launch_paged_decode_as<64, true>(d, s) : launch_paged_decode_as<64, false>(d, s);
+        const bool two = (long long)p.c.max_rows * p.G > 8;
+        if (c.D == 128) {
+            if (s8) return two ? launch_paged_decode_as<128, true, 2>(d, s) : launch_paged_decode_as<128, true, 1>(d, s);
+            return two ? launch_paged_decode_as<128, false, 2>(d, s) : launch_paged_decode_as<128, false, 1>(d, s);
+        }
+        if (s8) return two ? launch_paged_decode_as<64, true, 2>(d, s) : launch_paged_decode_as<64, true, 1>(d, s);
+        return two ? launch_paged_decode_as<64, false, 2>(d, s) : launch_paged_decode_as<64, false, 1>(d, s);
     }
     const dim3 grid((unsigned)a.T, (unsigned)((a.H + 3) / 4));
     if (c.D == 128) s8 ? paged_rows_kernel<128, true><<<grid, 128, 0, s>>>(p) : paged_rows_kernel<128, false><<<grid, 128, 0, s>>>(p);

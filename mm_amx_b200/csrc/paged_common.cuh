@@ -35,6 +35,12 @@ __device__ __forceinline__ void mma_bf16_16816(float (&c)[4], unsigned a0, unsig
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// an 8 x 8 matrix of 16-bit values, two neighbours of row lane / 4 in each lane -> its transpose in the same form
+__device__ __forceinline__ unsigned transpose8x8(unsigned v) {
+    unsigned r;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+    return r;
+}
 __device__ __forceinline__ unsigned pack2_bf16(float lo, float hi) { return pack_bf16x2(lo, hi); }
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;

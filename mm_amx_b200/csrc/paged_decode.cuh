@@ -5,8 +5,9 @@
 // pieces, one per CTA, whatever the lengths: with a piece per pair the longest sequence would decide.  A CTA walks its piece pair by pair; a pair that
 // lies in several pieces leaves a sub-state (maximum, sum, unnormalised values) per piece, which paged_combine_kernel merges.
 // Inside a CTA four warps take 16-token blocks of a unit each, with rings of their own filled by cp.async, and meet at the end of a pair.  The
-// next pair's first blocks are on their way before that.  Scores and values go through mma.sync.m16n8k16: the packed rows are the 16 rows, so K and V
-// cross shared memory once for all of them (bytes bound it: 23 per clock and SM at HBM speed; tcgen05 would work on 128 rows).
+// next pair's first blocks are on their way before that.  Scores and values go through mma.sync.m16n8k16 with tokens (then components) as the 16 rows and
+// the packed rows as one or two operands of 8 columns (with the packed rows as the 16 rows, most groups leave half of every product empty); the
+// probabilities turn from one form into the other by movmatrix.  (tcgen05 would work on 128 rows; bytes bound this: 23 per clock and SM at HBM speed.)
 // 8 bits: bytes become bf16 of (value / 64), exactly, in two instructions a pair; the page's factors go into the scores and into the probabilities.
 #pragma once
 #include "paged_common.cuh"
@@ -15,16 +16,19 @@ namespace b200fc {
 
 namespace {
 
-constexpr int DEC_WARPS = 4, DEC_THREADS = 128, DEC_STAGES = 3;
+constexpr int DEC_WARPS = 4, DEC_THREADS = 128;
 constexpr int DEC_UNIT = 64;                       // tokens of a unit: 16 per warp
 
-template <int D, bool S8> struct DecSmem {
+template <int D, bool S8, int NT> struct DecSmem {
     static constexpr int ROW = D * (S8 ? 1 : 2), CHUNKS = ROW / 16;
     static constexpr int BLOCK = 16 * ROW;                              // 16 tokens of K (or V)
-    static constexpr int STAGE = 2 * BLOCK, RING = DEC_WARPS * DEC_STAGES * STAGE;
-    static constexpr int STATE = 2 * 16 * D * 4;                        // values of two warps
+    static constexpr int CTAS = D == 128 ? (S8 ? 3 : 2) : (S8 ? 4 : 3);  // per SM
+    static constexpr int STAGES = D == 128 ? 3 : 4;
+    static constexpr int STAGE = 2 * BLOCK, RING = DEC_WARPS * STAGES * STAGE;
+    static constexpr int ROW_STATE = D + (NT == 1 ? 8 : 0), WARP_STATE = 8 * NT * ROW_STATE;   // floats: a packed row's values, a warp's
+    static constexpr int STATE = 2 * WARP_STATE * 4;
     static constexpr int BYTES = RING + STATE + DEC_WARPS * 16 * 8 + 128;
-    static constexpr int CTAS = D == 128 ? (S8 ? 3 : 2) : 4;            // per SM
+    static_assert(CTAS * (BYTES + 1024 + 256) <= 233472, "resident together (1 KB of each CTA is the system's)");
 };
 // byte offset of 16-byte chunk c of token row r inside a block: eight rows of one chunk lie in eight different bank groups
 template <int CHUNKS> __device__ __forceinline__ int dec_place(int r, int c) {
@@ -55,47 +59,57 @@ __device__ __forceinline__ bool dec_seq(const PagedAttn& p, int b, DecSeq* q) {
     return ok;
 }
 
-template <int D, bool S8>
-__global__ void __launch_bounds__(DEC_THREADS, DecSmem<D, S8>::CTAS) paged_decode_kernel(const DecParams p) {
-    using SM = DecSmem<D, S8>;
-    constexpr int CHUNKS = SM::CHUNKS, KSTEPS = D / 16;
+template <int D, bool S8, int NT>
+__global__ void __launch_bounds__(DEC_THREADS, DecSmem<D, S8, NT>::CTAS) paged_decode_kernel(const DecParams p) {
+    using SM = DecSmem<D, S8, NT>;
+    constexpr int CHUNKS = SM::CHUNKS, KSTEPS = D / 16, DEC_STAGES = SM::STAGES;
     extern __shared__ unsigned char dec_smem_raw[];
-    __shared__ int warp_sum[DEC_WARPS], found[4], odd_value;
+    __shared__ int warp_sum[DEC_WARPS], odd_value;
+    __shared__ struct { DecSeq seq; int b, hk, j; } first;
     unsigned char* smem = dec_smem_raw + (((smem_u32(dec_smem_raw) + 127u) & ~127u) - smem_u32(dec_smem_raw));
-    float* st_o = (float*)(smem + SM::RING);                  // [2][16][D]
-    float* st_ml = st_o + 2 * 16 * D;                         // [warp][16][2]
+    float* st_o = (float*)(smem + SM::RING);                  // states of two warps
+    float* st_ml = st_o + 2 * SM::WARP_STATE;                         // [warp][16][2]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
     const PagedAttn& a = p.a;
     const int Hkv = a.c.Hkv, B = a.c.B;
 
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
 
-    // ---- units of all sequences; CTA 0 leaves their running sum for the combining kernel ----
-    long long total = 0;
-    for (int b0 = 0; b0 < B; b0 += DEC_THREADS) {
+    // ---- units of all sequences, 128 at a time; CTA 0 leaves their running sum for the combining kernel ----
+    DecSeq mine;                                              // of the thread's sequence of the round at hand
+    int units_of_mine = 0, in_front = 0, round_units = 0;     // in_front: units of the round's sequences before the thread's
+    auto scan_round = [&](int b0) {
         const int b = b0 + threadIdx.x;
-        DecSeq q;
-        int n = 0;
+        units_of_mine = 0;
+        bool ok = true;
         if (b < B) {
-            if (!dec_seq(a, b, &q) && blockIdx.x == 0) report_paged(a.c);
-            n = q.units;
-            if (n == 0 && q.s.rows > 0 && b % gridDim.x == blockIdx.x) zero_rows<D>(a, q.s);
+            ok = dec_seq(a, b, &mine);
+            units_of_mine = mine.units;
         }
-        int upto = n;
+        int upto = units_of_mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int u = __shfl_up_sync(0xffffffffu, upto, o);
             if (lane >= o) upto += u;
         }
+        __syncthreads();
         if (lane == 31) warp_sum[warp] = upto;
         __syncthreads();
-        int before = 0, all = 0;
+        in_front = upto - units_of_mine;
+        round_units = 0;
 #pragma unroll
-        for (int w = 0; w < DEC_WARPS; w++) { before += w < warp ? warp_sum[w] : 0; all += warp_sum[w]; }
-        if (blockIdx.x == 0 && b < B) p.prefix[b] = total + before + upto - n;
-        total += all;
-        __syncthreads();
+        for (int w = 0; w < DEC_WARPS; w++) { in_front += w < warp ? warp_sum[w] : 0; round_units += warp_sum[w]; }
+        return ok;
+    };
+    long long total = 0;
+    for (int b0 = 0; b0 < B; b0 += DEC_THREADS) {
+        const int b = b0 + threadIdx.x;
+        if (!scan_round(b0) && blockIdx.x == 0) report_paged(a.c);
+        if (b < B) {
+            if (units_of_mine == 0 && mine.s.rows > 0 && b % gridDim.x == blockIdx.x) zero_rows<D>(a, mine.s);
+            if (blockIdx.x == 0) p.prefix[b] = total + in_front;
+        }
+        total += round_units;
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) p.prefix[B] = total;
     total *= Hkv;
@@ -104,33 +118,20 @@ __global__ void __launch_bounds__(DEC_THREADS, DecSmem<D, S8>::CTAS) paged_decod
     const long long u0 = total * blockIdx.x / pieces, u1 = total * (blockIdx.x + 1) / pieces;
 
     // ---- the sequence that unit u0 belongs to ----
-    long long seen = 0;
-    for (int b0 = 0; b0 < B; b0 += DEC_THREADS) {
-        const int b = b0 + threadIdx.x;
-        DecSeq q;
-        int n = 0;
-        if (b < B) { dec_seq(a, b, &q); n = q.units; }
-        int upto = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += u;
+    for (long long b0 = 0, seen = 0; b0 < B; b0 += DEC_THREADS) {
+        if (B > DEC_THREADS) scan_round((int)b0);             // (else the one round's numbers are still there)
+        const long long lo = (seen + in_front) * Hkv;
+        if (units_of_mine && u0 >= lo && u0 < lo + (long long)units_of_mine * Hkv) {
+            first.seq = mine;
+            first.b = (int)b0 + threadIdx.x; first.hk = (int)((u0 - lo) / units_of_mine); first.j = (int)((u0 - lo) % units_of_mine);
         }
-        if (lane == 31) warp_sum[warp] = upto;
-        __syncthreads();
-        int before = 0, all = 0;
-#pragma unroll
-        for (int w = 0; w < DEC_WARPS; w++) { before += w < warp ? warp_sum[w] : 0; all += warp_sum[w]; }
-        const long long lo = (seen + before + upto - n) * Hkv, hi = lo + (long long)n * Hkv;
-        if (n && u0 >= lo && u0 < hi) { found[0] = b; found[1] = (int)((u0 - lo) / n); found[2] = (int)((u0 - lo) % n); }
-        seen += all;
-        __syncthreads();
+        seen += round_units;
         if (u0 < seen * Hkv) break;
     }
-    int b = found[0], hk = found[1], j0 = found[2];
+    __syncthreads();
+    int b = first.b, hk = first.hk, j0 = first.j;
     long long left = u1 - u0;
-    DecSeq cur;
-    dec_seq(a, b, &cur);
+    DecSeq cur = first.seq;
     unsigned char* ring = smem + warp * DEC_STAGES * SM::STAGE;
 
     // One run of units [j0, j1) of a pair.  A warp's blocks are 4 j + warp.
@@ -152,20 +153,25 @@ __global__ void __launch_bounds__(DEC_THREADS, DecSmem<D, S8>::CTAS) paged_decod
         kbase = a.c.k + (long long)hk * a.c.head_stride;
         vbase = a.c.v + (long long)hk * a.c.head_stride;
     };
+    const int lane_row = lane / CHUNKS, lane_chunk = lane % CHUNKS;
+    constexpr int ROWS_AT_ONCE = 32 / CHUNKS;               // token rows of one copy instruction of the warp
+    const long long lane_off = (long long)lane_row * a.c.token_stride + lane_chunk * 16, step = (long long)ROWS_AT_ONCE * a.c.token_stride;
     auto issue = [&](int j) {
         const int i = 4 * j + warp, page = next_page, slot = (j - j0) % DEC_STAGES;
         if (j < j1) {
             const int tok0 = key_block(cur.kb, i) << 4;
-            unsigned char* st = ring + slot * SM::STAGE;
-            const long long at = (long long)max(page, 0) * a.c.page_stride + (long long)(tok0 & ((1 << a.c.page_shift) - 1)) * a.c.token_stride;
+            const unsigned st = smem_u32(ring) + slot * SM::STAGE;
+            const long long at = (long long)max(page, 0) * a.c.page_stride + (long long)(tok0 & ((1 << a.c.page_shift) - 1)) * a.c.token_stride + lane_off;
+            const unsigned char *ks = kbase + at, *vs = vbase + at;
+            const bool all = page >= 0 && tok0 + 16 <= cur.kb.end && (tok0 >= cur.kb.begin || tok0 + 16 <= cur.kb.sink_end);
 #pragma unroll
-            for (int n = 0; n < 16 * CHUNKS / 32; n++) {
-                const int u = n * 32 + lane, row = u / CHUNKS, c = u % CHUNKS, tok = tok0 + row;
-                const bool ok = page >= 0 && tok < cur.kb.end && (tok >= cur.kb.begin || tok < cur.kb.sink_end);
-                const unsigned dst = smem_u32(st) + dec_place<CHUNKS>(row, c);
-                const long long off = ok ? at + (long long)row * a.c.token_stride + c * 16 : 0;
-                cp_async16_or_zero(dst, kbase + off, ok);
-                cp_async16_or_zero(dst + SM::BLOCK, vbase + off, ok);
+            for (int n = 0; n < 16 / ROWS_AT_ONCE; n++) {
+                const int row = n * ROWS_AT_ONCE + lane_row, tok = tok0 + row;
+                const bool ok = all || (page >= 0 && tok < cur.kb.end && (tok >= cur.kb.begin || tok < cur.kb.sink_end));
+                const unsigned dst = st + dec_place<CHUNKS>(row, lane_chunk);
+                cp_async16_or_zero(dst, ok ? ks : kbase, ok);
+                cp_async16_or_zero(dst + SM::BLOCK, ok ? vs : vbase, ok);
+                ks += step; vs += step;
             }
         }
         have = page >= 0 ? have | 1u << slot : have & ~(1u << slot);
@@ -189,34 +195,35 @@ __global__ void __launch_bounds__(DEC_THREADS, DecSmem<D, S8>::CTAS) paged_decod
         const SeqRows s = cur.s;
         const KeyBlocks kb = cur.kb;
         const int rows = s.rows * a.G, units = cur.units, run0 = j0, run1 = j1, at_b = b, at_hk = hk;
-        // ---- Q: packed row i = (row i / G, head i % G of the group); rows past the last one are zeros ----
-        unsigned qa[KSTEPS][4];
-        int place[2];
-        {
-            const unsigned char* qp[2];
-            bool ok[2];
+        // ---- Q as the 8-column operand: column n of tile nt = packed row 8 nt + n = (row / G, head % G of the group); zeros past the last one ----
+        unsigned qb[NT][KSTEPS][2];
 #pragma unroll
-            for (int r = 0; r < 2; r++) {
-                const int i = g + 8 * r, row = i / a.G;
-                ok[r] = i < rows;
-                place[r] = s.len - s.rows + row;
-                qp[r] = a.q + (long long)(s.row0 + row) * a.q_rs + (long long)(hk * a.G + i - row * a.G) * a.q_hs;
-            }
+        for (int nt = 0; nt < NT; nt++) {
+            const int i = 8 * nt + g, row = i / a.G;
+            const bool ok = i < rows;
+            const unsigned char* qp = a.q + (long long)(s.row0 + (ok ? row : 0)) * a.q_rs + (long long)(hk * a.G + (ok ? i - row * a.G : 0)) * a.q_hs;
 #pragma unroll
             for (int ks = 0; ks < KSTEPS; ks++) {
-                // (8 bits: a k-step's columns are permuted as the bytes of a chunk come out of ldmatrix)
+                // (8 bits: the components of a k-step are permuted as the bytes of a chunk come out of ldmatrix)
                 const int d0 = ks * 16 + (S8 ? 4 * t : 2 * t), d1 = d0 + (S8 ? 2 : 8);
-#pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    qa[ks][r] = ok[r] ? __ldg((const unsigned*)(qp[r] + d0 * 2)) : 0u;
-                    qa[ks][2 + r] = ok[r] ? __ldg((const unsigned*)(qp[r] + d1 * 2)) : 0u;
-                }
+                qb[nt][ks][0] = ok ? __ldg((const unsigned*)(qp + d0 * 2)) : 0u;
+                qb[nt][ks][1] = ok ? __ldg((const unsigned*)(qp + d1 * 2)) : 0u;
             }
         }
-        float o[D / 8][4];
+        // a lane's scores and values belong to packed rows 8 nt + 2 t + r
+        int place[NT][2];
+        float o[NT][D / 16][4], m_run[NT][2], l_run[NT][2];
 #pragma unroll
-        for (int i = 0; i < D / 8; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
-        float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.0f, 0.0f};
+        for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+            for (int i = 0; i < D / 16; i++) o[nt][i][0] = o[nt][i][1] = o[nt][i][2] = o[nt][i][3] = 0.0f;
+#pragma unroll
+            for (int r = 0; r < 2; r++) {
+                place[nt][r] = s.len - s.rows + (8 * nt + 2 * t + r) / a.G;
+                m_run[nt][r] = -INFINITY;
+                l_run[nt][r] = 0.0f;
+            }
+        }
         const int place_lo = s.len - s.rows, place_hi = s.len - 1;
         bool odd = false;
 
@@ -225,7 +232,7 @@ __global__ void __launch_bounds__(DEC_THREADS, DecSmem<D, S8>::CTAS) paged_decod
             issue(j + DEC_STAGES - 1);
             cp_async_wait<DEC_STAGES - 1>();
             __syncwarp();
-            const int slot = (j - run0) % DEC_STAGES, i = 4 * j + warp;
+            const int slot = (j - run0) % DEC_STAGES, i = 4 * j + warp, mi = lane >> 3;
             const unsigned kst = smem_u32(ring) + slot * SM::STAGE, vst = kst + SM::BLOCK;
             const int tok0 = key_block(kb, i) << 4;
             float fk = a.scale_log2e, fv = 1.0f;
@@ -235,106 +242,123 @@ __global__ void __launch_bounds__(DEC_THREADS, DecSmem<D, S8>::CTAS) paged_decod
                 fk *= 64.0f * a.scale_log2e;
                 fv *= 64.0f;
             }
-            float sc[2][4] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
-            if constexpr (!S8) {
-                const int mi = lane >> 3, tok = (mi >> 1) * 8 + (lane & 7);
+            // ---- S = K Q^T: 16 tokens x 8 rows; two chains of products ----
+            float sc[NT][4];
+            {
+                float part[NT][2][4];
 #pragma unroll
-                for (int ks = 0; ks < KSTEPS; ks++) {
-                    unsigned kr[4];
-                    ldsm_x4(kr, kst + dec_place<CHUNKS>(tok, 2 * ks + (mi & 1)));
-                    mma_bf16_16816(sc[0], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], kr[0], kr[1]);
-                    mma_bf16_16816(sc[1], qa[ks][0], qa[ks][1], qa[ks][2], qa[ks][3], kr[2], kr[3]);
-                }
-            } else {
-                const int mi = lane >> 3, tok = (mi >> 1) * 8 + (lane & 7);
+                for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int k2 = 0; k2 < KSTEPS / 2; k2++) {
-                    unsigned kr[4];                       // [tokens 0-7, 8-15][two chunks of 16 components]
-                    ldsm_x4(kr, kst + dec_place<CHUNKS>(tok, 2 * k2 + (mi & 1)));
+                    for (int e = 0; e < 8; e++) part[nt][e >> 2][e & 3] = 0.0f;
+                const int tok = (mi & 1) * 8 + (lane & 7);
+                if constexpr (!S8) {
 #pragma unroll
-                    for (int h = 0; h < 2; h++)
+                    for (int ks = 0; ks < KSTEPS; ks++) {
+                        unsigned kr[4];                       // tokens 0-7, 8-15 of the first 8 components, then of the second
+                        ldsm_x4(kr, kst + dec_place<CHUNKS>(tok, 2 * ks + (mi >> 1)));
+#pragma unroll
+                        for (int nt = 0; nt < NT; nt++) mma_bf16_16816(part[nt][ks & 1], kr[0], kr[1], kr[2], kr[3], qb[nt][ks][0], qb[nt][ks][1]);
+                    }
+                } else {
+#pragma unroll
+                    for (int k2 = 0; k2 < KSTEPS / 2; k2++) {
+                        unsigned kr[4];                       // tokens 0-7, 8-15 of one chunk of 16 components, then of the next
+                        ldsm_x4(kr, kst + dec_place<CHUNKS>(tok, 2 * k2 + (mi >> 1)));
 #pragma unroll
                         for (int e = 0; e < 2; e++) {
-                            const unsigned w = kr[2 * h + e] ^ 0x80808080u;
-                            mma_bf16_16816(sc[h], qa[2 * k2 + e][0], qa[2 * k2 + e][1], qa[2 * k2 + e][2], qa[2 * k2 + e][3],
-                                           u8x2_to_bf16x2_64th(w, 0x4140), u8x2_to_bf16x2_64th(w, 0x4342));
+                            const unsigned w0 = kr[2 * e] ^ 0x80808080u, w1 = kr[2 * e + 1] ^ 0x80808080u;
+                            const unsigned a0 = u8x2_to_bf16x2_64th(w0, 0x4140), a1 = u8x2_to_bf16x2_64th(w1, 0x4140);
+                            const unsigned a2 = u8x2_to_bf16x2_64th(w0, 0x4342), a3 = u8x2_to_bf16x2_64th(w1, 0x4342);
+#pragma unroll
+                            for (int nt = 0; nt < NT; nt++) mma_bf16_16816(part[nt][e], a0, a1, a2, a3, qb[nt][2 * k2 + e][0], qb[nt][2 * k2 + e][1]);
                         }
+                    }
                 }
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++) sc[nt][c] = (part[nt][0][c] + part[nt][1][c]) * fk;
             }
-            // ---- online softmax (exp2 domain) ----
+            // ---- online softmax (exp2 domain): a lane's tokens are tok0 + g and tok0 + g + 8 ----
             const bool there = have >> slot & 1;
             const bool whole = there && tok0 + 15 <= place_lo && (tok0 + 15 < a.sinks || a.window == 0 || tok0 > place_hi - a.window);
-            float bm[2] = {-INFINITY, -INFINITY};
+            if (!whole) {
 #pragma unroll
-            for (int tt = 0; tt < 2; tt++)
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int c = 0; c < 4; c++)
+                        if (!(there && key_visible(tok0 + g + (c >> 1) * 8, place[nt][c & 1], a.window, a.sinks))) sc[nt][c] = -INFINITY;
+            }
+            float top[NT][2];
+            bool rose = false;
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int r = 0; r < 2; r++) {
+                    float x = fmaxf(sc[nt][r], sc[nt][2 + r]);
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                    top[nt][r] = fmaxf(m_run[nt][r], x);
+                    rose = rose || top[nt][r] > m_run[nt][r];
+                }
+            if (__any_sync(0xffffffffu, rose)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    float f[2];
+#pragma unroll
+                    for (int r = 0; r < 2; r++) {
+                        f[r] = top[nt][r] == -INFINITY ? 1.0f : exp2_approx(m_run[nt][r] - top[nt][r]);
+                        m_run[nt][r] = top[nt][r];
+                        l_run[nt][r] *= f[r];
+                    }
+#pragma unroll
+                    for (int n = 0; n < D / 16; n++)
+#pragma unroll
+                        for (int c = 0; c < 4; c++) o[nt][n][c] *= f[c & 1];
+                }
+            }
+            unsigned pb[NT][2];
+#pragma unroll
+            for (int nt = 0; nt < NT; nt++) {
+                float e[4];
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
-                    const int tok = tok0 + tt * 8 + 2 * t + (c & 1);
-                    float x = sc[tt][c] * fk;
-                    if (!whole && !(there && key_visible(tok, place[c >> 1], a.window, a.sinks))) x = -INFINITY;
-                    sc[tt][c] = x;
-                    bm[c >> 1] = fmaxf(bm[c >> 1], x);
+                    const float x = sc[nt][c];
+                    e[c] = whole || x != -INFINITY ? exp2_approx(x - m_run[nt][c & 1]) : 0.0f;
+                    l_run[nt][c & 1] += e[c];
+                    if (S8) e[c] = whole || x != -INFINITY ? e[c] * fv : 0.0f;
                 }
-#pragma unroll
-            for (int r = 0; r < 2; r++) {
-                bm[r] = fmaxf(bm[r], __shfl_xor_sync(0xffffffffu, bm[r], 1));
-                bm[r] = fmaxf(bm[r], __shfl_xor_sync(0xffffffffu, bm[r], 2));
+                // (token g, rows 2 t, 2 t + 1) -> (row g, tokens 2 t, 2 t + 1)
+                pb[nt][0] = transpose8x8(pack2_bf16(e[0], e[1]));
+                pb[nt][1] = transpose8x8(pack2_bf16(e[2], e[3]));
             }
-            float corr[2];
-#pragma unroll
-            for (int r = 0; r < 2; r++) {
-                const float m_new = fmaxf(m_run[r], bm[r]);
-                corr[r] = m_new == -INFINITY ? 1.0f : exp2_approx(m_run[r] - m_new);
-                m_run[r] = m_new;
-                l_run[r] *= corr[r];
-            }
-#pragma unroll
-            for (int tt = 0; tt < 2; tt++)
-#pragma unroll
-                for (int c = 0; c < 4; c++) {
-                    const float x = sc[tt][c];
-                    const float e = whole || x != -INFINITY ? exp2_approx(x - m_run[c >> 1]) : 0.0f;
-                    l_run[c >> 1] += e;
-                    sc[tt][c] = S8 ? (whole || x != -INFINITY ? e * fv : 0.0f) : e;
-                }
-            const unsigned pa0 = pack2_bf16(sc[0][0], sc[0][1]), pa1 = pack2_bf16(sc[0][2], sc[0][3]);
-            const unsigned pa2 = pack2_bf16(sc[1][0], sc[1][1]), pa3 = pack2_bf16(sc[1][2], sc[1][3]);
-            // ---- O = O * corr + P V ----
-            const int mi = lane >> 3;
+            // ---- O^T += V^T P^T: 16 components x 8 rows ----
             if constexpr (!S8) {
-                const int tok = (mi & 1) * 8 + (lane & 7);
+                const int tok = (mi >> 1) * 8 + (lane & 7);
                 unsigned worst = 0;
 #pragma unroll
-                for (int c2 = 0; c2 < CHUNKS / 2; c2++) {
-                    unsigned vr[4];
-                    ldsm_x4_trans(vr, vst + dec_place<CHUNKS>(tok, 2 * c2 + (mi >> 1)));
-                    if (!whole) {
+                for (int n = 0; n < D / 16; n++) {
+                    unsigned vr[4];                           // components 0-7, 8-15 of tokens 0-7, then of tokens 8-15
+                    ldsm_x4_trans(vr, vst + dec_place<CHUNKS>(tok, 2 * n + (mi & 1)));
+                    if (!whole) worst |= not_finite2(vr[0]) | not_finite2(vr[1]) | not_finite2(vr[2]) | not_finite2(vr[3]);
 #pragma unroll
-                        for (int q = 0; q < 4; q++) worst |= not_finite2(vr[q]);
-                    }
-#pragma unroll
-                    for (int h2 = 0; h2 < 2; h2++) {
-                        float (&acc)[4] = o[2 * c2 + h2];
-                        acc[0] *= corr[0]; acc[1] *= corr[0]; acc[2] *= corr[1]; acc[3] *= corr[1];
-                        mma_bf16_16816(acc, pa0, pa1, pa2, pa3, vr[2 * h2], vr[2 * h2 + 1]);
-                    }
+                    for (int nt = 0; nt < NT; nt++) mma_bf16_16816(o[nt][n], vr[0], vr[1], vr[2], vr[3], pb[nt][0], pb[nt][1]);
                 }
                 odd = odd || worst != 0;
             } else {
                 const int tok = (mi & 1) * 8 + (lane & 7);
 #pragma unroll
-                for (int c2 = 0; c2 < CHUNKS / 2; c2++) {
-                    unsigned vr[4];                       // [two chunks][tokens 0-7, 8-15]: a register holds components 2 g, 2 g + 1 of two tokens
-                    ldsm_x4_trans(vr, vst + dec_place<CHUNKS>(tok, 2 * c2 + (mi >> 1)));
+                for (int n2 = 0; n2 < D / 32; n2++) {
+                    unsigned vr[4];                           // two chunks of (tokens 0-7, 8-15); a register holds components 2 g, 2 g + 1 of two tokens
+                    ldsm_x4_trans(vr, vst + dec_place<CHUNKS>(tok, 2 * n2 + (mi >> 1)));
 #pragma unroll
-                    for (int h2 = 0; h2 < 2; h2++) {
-                        const unsigned w0 = vr[2 * h2] ^ 0x80808080u, w1 = vr[2 * h2 + 1] ^ 0x80808080u;
+                    for (int e = 0; e < 2; e++) {
+                        const unsigned w0 = vr[2 * e] ^ 0x80808080u, w1 = vr[2 * e + 1] ^ 0x80808080u;
+                        const unsigned a0 = u8x2_to_bf16x2_64th(w0, 0x4240), a1 = u8x2_to_bf16x2_64th(w0, 0x4341);
+                        const unsigned a2 = u8x2_to_bf16x2_64th(w1, 0x4240), a3 = u8x2_to_bf16x2_64th(w1, 0x4341);
 #pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            float (&acc)[4] = o[2 * (2 * c2 + h2) + e];
-                            acc[0] *= corr[0]; acc[1] *= corr[0]; acc[2] *= corr[1]; acc[3] *= corr[1];
-                            mma_bf16_16816(acc, pa0, pa1, pa2, pa3, u8x2_to_bf16x2_64th(w0, e ? 0x4341 : 0x4240), u8x2_to_bf16x2_64th(w1, e ? 0x4341 : 0x4240));
-                        }
+                        for (int nt = 0; nt < NT; nt++) mma_bf16_16816(o[nt][2 * n2 + e], a0, a1, a2, a3, pb[nt][0], pb[nt][1]);
                     }
                 }
             }
@@ -356,52 +380,59 @@ __global__ void __launch_bounds__(DEC_THREADS, DecSmem<D, S8>::CTAS) paged_decod
             for (int j = 0; j < DEC_STAGES - 1; j++) issue(j);
         }
 
-        // ---- the four warps' states ----
+        // (the combining kernel may come up now: earlier its CTAs would only take places)
+        else asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+        // ---- the four warps' states: values by lane (each warp's lanes hold the same places), maxima and sums by row ----
 #pragma unroll
-        for (int r = 0; r < 2; r++) {
-            l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 1);
-            l_run[r] += __shfl_xor_sync(0xffffffffu, l_run[r], 2);
-        }
+        for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+            for (int r = 0; r < 2; r++)
+#pragma unroll
+                for (int x = 4; x < 32; x *= 2) l_run[nt][r] += __shfl_xor_sync(0xffffffffu, l_run[nt][r], x);
         auto put_state = [&](float* dst) {
 #pragma unroll
-            for (int i = 0; i < D / 8; i++) {
-                *(float2*)(dst + g * D + i * 8 + 2 * t) = make_float2(o[i][0], o[i][1]);
-                *(float2*)(dst + (g + 8) * D + i * 8 + 2 * t) = make_float2(o[i][2], o[i][3]);
-            }
+            for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                for (int n = 0; n < D / 16; n++) ((float4*)dst)[(nt * (D / 16) + n) * 32 + lane] = make_float4(o[nt][n][0], o[nt][n][1], o[nt][n][2], o[nt][n][3]);
         };
         auto put_ml = [&](int w) {
-            if (t == 0) {
-                *(float2*)(st_ml + (w * 16 + g) * 2) = make_float2(m_run[0], l_run[0]);
-                *(float2*)(st_ml + (w * 16 + g + 8) * 2) = make_float2(m_run[1], l_run[1]);
-            }
+            if (g == 0)
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                    for (int r = 0; r < 2; r++) *(float2*)(st_ml + (w * 16 + 8 * nt + 2 * t + r) * 2) = make_float2(m_run[nt][r], l_run[nt][r]);
         };
         auto take_state = [&](const float* src, int w) {
-            float f[2], e[2];
 #pragma unroll
-            for (int r = 0; r < 2; r++) {
-                const float2 ml = *(const float2*)(st_ml + (w * 16 + g + 8 * r) * 2);
-                const float m = fmaxf(m_run[r], ml.x);
-                f[r] = m_run[r] == -INFINITY ? 0.0f : exp2_approx(m_run[r] - m);
-                e[r] = ml.x == -INFINITY ? 0.0f : exp2_approx(ml.x - m);
-                l_run[r] = l_run[r] * f[r] + ml.y * e[r];
-                m_run[r] = m;
-            }
+            for (int nt = 0; nt < NT; nt++) {
+                float f[2], e[2];
 #pragma unroll
-            for (int i = 0; i < D / 8; i++) {
-                const float2 x = *(const float2*)(src + g * D + i * 8 + 2 * t), y = *(const float2*)(src + (g + 8) * D + i * 8 + 2 * t);
-                o[i][0] = o[i][0] * f[0] + x.x * e[0]; o[i][1] = o[i][1] * f[0] + x.y * e[0];
-                o[i][2] = o[i][2] * f[1] + y.x * e[1]; o[i][3] = o[i][3] * f[1] + y.y * e[1];
+                for (int r = 0; r < 2; r++) {
+                    const float2 ml = *(const float2*)(st_ml + (w * 16 + 8 * nt + 2 * t + r) * 2);
+                    const float m = fmaxf(m_run[nt][r], ml.x);
+                    f[r] = m_run[nt][r] == -INFINITY ? 0.0f : exp2_approx(m_run[nt][r] - m);
+                    e[r] = ml.x == -INFINITY ? 0.0f : exp2_approx(ml.x - m);
+                    l_run[nt][r] = l_run[nt][r] * f[r] + ml.y * e[r];
+                    m_run[nt][r] = m;
+                }
+#pragma unroll
+                for (int n = 0; n < D / 16; n++) {
+                    const float4 x = ((const float4*)src)[(nt * (D / 16) + n) * 32 + lane];
+                    o[nt][n][0] = o[nt][n][0] * f[0] + x.x * e[0]; o[nt][n][1] = o[nt][n][1] * f[1] + x.y * e[1];
+                    o[nt][n][2] = o[nt][n][2] * f[0] + x.z * e[0]; o[nt][n][3] = o[nt][n][3] * f[1] + x.w * e[1];
+                }
             }
         };
         if (threadIdx.x == 0) odd_value = 0;
         __syncthreads();                                  // (the previous pair's states have been read)
         if (odd) odd_value = 1;
         put_ml(warp);
-        if (warp >= 2) put_state(st_o + (warp - 2) * 16 * D);
+        if (warp >= 2) put_state(st_o + (warp - 2) * SM::WARP_STATE);
         __syncthreads();
-        if (warp < 2) take_state(st_o + warp * 16 * D, warp + 2);
+        if (warp < 2) take_state(st_o + warp * SM::WARP_STATE, warp + 2);
         __syncwarp();
-        if (warp == 1) { put_ml(1); put_state(st_o + 16 * D); }
+        if (warp == 1) { put_ml(1); put_state(st_o + SM::WARP_STATE); }
         __syncthreads();
         const bool split = run0 > 0 || run1 < units;
         const size_t sub = ((size_t)blockIdx.x * 2 + (run0 > 0 ? 0 : 1)) * 16;
@@ -411,29 +442,34 @@ __global__ void __launch_bounds__(DEC_THREADS, DecSmem<D, S8>::CTAS) paged_decod
                 row_state<D, S8>(a, at_b, s, i / a.G, at_hk * a.G + i % a.G, kb, 4 * run0, min(4 * run1, kb.count), split ? p.ws_o + (sub + i) * D : nullptr,
                                  split ? p.ws_ml + (sub + i) * 2 : nullptr);
         } else if (warp == 0) {
-            take_state(st_o + 16 * D, 1);
+            take_state(st_o + SM::WARP_STATE, 1);
+            // through shared memory once more (where warp 0's state would have been), so that rows are stored in whole
 #pragma unroll
-            for (int r = 0; r < 2; r++) {
-                const int i = g + 8 * r, row = i / a.G;
-                if (i >= rows) continue;
-                float* wo = p.ws_o + (sub + i) * D;
-                unsigned char* out = a.out + (long long)(s.row0 + row) * a.o_rs + (long long)(at_hk * a.G + i - row * a.G) * a.o_hs;
-                const float inv = l_run[r] != 0.0f ? 1.0f / l_run[r] : 0.0f;
-                if (split && t == 0) *(float2*)(p.ws_ml + (sub + i) * 2) = make_float2(m_run[r], l_run[r]);
+            for (int nt = 0; nt < NT; nt++)
 #pragma unroll
-                for (int n = 0; n < D / 8; n += 2) {
-                    // two runs of two neighbours, or (8 bits) four neighbours
-                    float x[4] = {o[n][2 * r], o[n][2 * r + 1], o[n + 1][2 * r], o[n + 1][2 * r + 1]};
-                    if (S8) { const float y = x[1]; x[1] = x[2]; x[2] = y; }
-                    const int d0 = S8 ? 8 * n + 4 * t : 8 * n + 2 * t, d1 = S8 ? d0 + 2 : d0 + 8;
-                    if (split) {
-                        *(float2*)(wo + d0) = make_float2(x[0], x[1]);
-                        *(float2*)(wo + d1) = make_float2(x[2], x[3]);
-                    } else {
-                        *(unsigned*)(out + 2 * d0) = pack2_bf16(x[0] * inv, x[1] * inv);
-                        *(unsigned*)(out + 2 * d1) = pack2_bf16(x[2] * inv, x[3] * inv);
+                for (int r = 0; r < 2; r++) {
+                    float* dst = st_o + (8 * nt + 2 * t + r) * SM::ROW_STATE;
+#pragma unroll
+                    for (int n = 0; n < D / 16; n++) {
+                        dst[16 * n + (S8 ? 2 * g : g)] = o[nt][n][r];
+                        dst[16 * n + (S8 ? 2 * g + 1 : g + 8)] = o[nt][n][2 + r];
+                    }
+                    if (g == 0) *(float2*)(st_ml + (8 * nt + 2 * t + r) * 2) = make_float2(m_run[nt][r], l_run[nt][r]);
+                }
+            __syncwarp();
+            for (int i = 0; i < rows; i++) {
+                const float2 ml = *(const float2*)(st_ml + i * 2);
+                const int row = i / a.G;
+#pragma unroll
+                for (int d = lane * 2; d < D; d += 64) {
+                    const float2 x = *(const float2*)(st_o + i * SM::ROW_STATE + d);
+                    if (split) *(float2*)(p.ws_o + (sub + i) * D + d) = x;
+                    else {
+                        const float inv = ml.y != 0.0f ? 1.0f / ml.y : 0.0f;
+                        *(unsigned*)(a.out + (long long)(s.row0 + row) * a.o_rs + (long long)(at_hk * a.G + i - row * a.G) * a.o_hs + 2 * d) = pack2_bf16(x.x * inv, x.y * inv);
                     }
                 }
+                if (split && lane == 0) *(float2*)(p.ws_ml + (sub + i) * 2) = ml;
             }
         }
         if (!more) break;
@@ -448,16 +484,15 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const DecParams p) {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const PagedAttn& a = p.a;
     const int b = blockIdx.x / a.c.Hkv, hk = blockIdx.x % a.c.Hkv, i = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    SeqRows s;
+    load_seq(a.c, b, &s);
     const long long before = p.prefix[b], n = p.prefix[b + 1] - before;
     if (n == 0) return;
     const long long total = p.prefix[a.c.B] * a.c.Hkv, x = before * a.c.Hkv + hk * n;
     const int pieces = dec_pieces(total, p.ctas, p.min_units);
     // the pieces of the pair's first and last unit
     const int c0 = (int)(((x + 1) * pieces - 1) / total), c1 = (int)(((x + n) * pieces - 1) / total);
-    if (c0 == c1) return;
-    SeqRows s;
-    load_seq(a.c, b, &s);
-    if (i >= s.rows * a.G) return;
+    if (c0 == c1 || i >= s.rows * a.G) return;
     // the first piece holds the pair's beginning unless it begins exactly there, in which case too it is a sub-state that goes on behind
     auto slot = [&](int c) { return ((size_t)c * 2 + (c == c0 ? 1 : 0)) * 16 + i; };
     constexpr int N = D / 32;
@@ -505,12 +540,12 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const DecParams p) {
     for (int e = 0; e < N; e += 2) *(unsigned*)(out + 2 * (lane * N + e)) = pack2_bf16(acc[e] * inv, acc[e + 1] * inv);
 }
 
-template <int D, bool S8>
+template <int D, bool S8, int NT>
 int launch_paged_decode_as(DecParams& p, cudaStream_t s) {
-    using SM = DecSmem<D, S8>;
+    using SM = DecSmem<D, S8, NT>;
     static std::atomic<unsigned long long> attr_devices{0};
     const int arc = once_per_device(attr_devices, [] {
-        B200FC_CUDA(cudaFuncSetAttribute(paged_decode_kernel<D, S8>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::BYTES));
+        B200FC_CUDA(cudaFuncSetAttribute(paged_decode_kernel<D, S8, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::BYTES));
         return (int)B200FC_OK;
     });
     if (arc) return arc;
@@ -532,7 +567,7 @@ int launch_paged_decode_as(DecParams& p, cudaStream_t s) {
     p.prefix = (long long*)(p.ws_ml + states * 2);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[0].val.programmaticStreamSerializationAllowed = getenv("X_NOPDL") ? 0 : 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)p.ctas);
     cfg.blockDim = dim3(DEC_THREADS);
@@ -540,7 +575,7 @@ int launch_paged_decode_as(DecParams& p, cudaStream_t s) {
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, paged_decode_kernel<D, S8>, (const DecParams)p);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, paged_decode_kernel<D, S8, NT>, (const DecParams)p);
     if (e == cudaSuccess) {
         count_launch();
         if (p.ctas > 1) {
