@@ -27,7 +27,7 @@ template <int D, bool S8, int NT> struct DecSmem {
     static constexpr int STAGE = 2 * BLOCK, RING = DEC_WARPS * STAGES * STAGE;
     static constexpr int ROW_STATE = D + (NT == 1 ? 8 : 0), WARP_STATE = 8 * NT * ROW_STATE;   // floats: a packed row's values, a warp's
     static constexpr int STATE = 2 * WARP_STATE * 4;
-    static constexpr int BYTES = RING + STATE + DEC_WARPS * 16 * 8 + 128;
+    static constexpr int BYTES = RING + STATE + DEC_WARPS * (16 * 8 + STAGES * 8) + 128;
     static_assert(CTAS * (BYTES + 1024 + 256) <= 233472, "resident together (1 KB of each CTA is the system's)");
 };
 // byte offset of 16-byte chunk c of token row r inside a block: eight rows of one chunk lie in eight different bank groups
@@ -138,7 +138,8 @@ __global__ void __launch_bounds__(DEC_THREADS, DecSmem<D, S8, NT>::CTAS) paged_d
     int j1 = (int)min((long long)cur.units, j0 + left);
     int next_page = -1;
     unsigned have = 0;                                     // slots of the ring whose block lies in a page of the pool
-    float kf[DEC_STAGES], vf[DEC_STAGES];                  // 8 bits: factors of the blocks in the ring
+    float* factors = (float*)(st_ml + DEC_WARPS * 16 * 2) + warp * DEC_STAGES * 2;     // 8 bits: of the blocks in the ring, k's and v's
+    const float* factor_src = lane == 0 ? a.c.k_scale : a.c.v_scale;
     const unsigned char *kbase, *vbase;
     auto look_up = [&](int j) {                            // page of the warp's block of unit j
         const int i = 4 * j + warp;
@@ -156,8 +157,9 @@ __global__ void __launch_bounds__(DEC_THREADS, DecSmem<D, S8, NT>::CTAS) paged_d
     const int lane_row = lane / CHUNKS, lane_chunk = lane % CHUNKS;
     constexpr int ROWS_AT_ONCE = 32 / CHUNKS;               // token rows of one copy instruction of the warp
     const long long lane_off = (long long)lane_row * a.c.token_stride + lane_chunk * 16, step = (long long)ROWS_AT_ONCE * a.c.token_stride;
+    int slot = 0;                                           // of the ring, that the next block goes to
     auto issue = [&](int j) {
-        const int i = 4 * j + warp, page = next_page, slot = (j - j0) % DEC_STAGES;
+        const int i = 4 * j + warp, page = next_page;
         if (j < j1) {
             const int tok0 = key_block(cur.kb, i) << 4;
             const unsigned st = smem_u32(ring) + slot * SM::STAGE;
@@ -175,15 +177,8 @@ __global__ void __launch_bounds__(DEC_THREADS, DecSmem<D, S8, NT>::CTAS) paged_d
             }
         }
         have = page >= 0 ? have | 1u << slot : have & ~(1u << slot);
-        if (S8) {
-            float fk = 0.0f, fv = 0.0f;
-            if (page >= 0) {
-                fk = __ldg(a.c.k_scale + page * a.c.scale_stride + hk);
-                fv = __ldg(a.c.v_scale + page * a.c.scale_stride + hk);
-            }
-#pragma unroll
-            for (int q = 0; q < DEC_STAGES; q++) if (q == slot) { kf[q] = fk; vf[q] = fv; }
-        }
+        if (S8 && lane < 2 && page >= 0) cp_async4(smem_u32(factors + 2 * slot + lane), factor_src + page * a.c.scale_stride + hk);
+        slot = slot + 1 == DEC_STAGES ? 0 : slot + 1;
         cp_async_commit();
         look_up(j + 1);
     };
@@ -232,15 +227,14 @@ __global__ void __launch_bounds__(DEC_THREADS, DecSmem<D, S8, NT>::CTAS) paged_d
             issue(j + DEC_STAGES - 1);
             cp_async_wait<DEC_STAGES - 1>();
             __syncwarp();
-            const int slot = (j - run0) % DEC_STAGES, i = 4 * j + warp, mi = lane >> 3;
-            const unsigned kst = smem_u32(ring) + slot * SM::STAGE, vst = kst + SM::BLOCK;
+            const int at = slot, i = 4 * j + warp, mi = lane >> 3;     // (the ring has gone round: the oldest block is where the next one goes)
+            const unsigned kst = smem_u32(ring) + at * SM::STAGE, vst = kst + SM::BLOCK;
             const int tok0 = key_block(kb, i) << 4;
             float fk = a.scale_log2e, fv = 1.0f;
             if (S8) {
-#pragma unroll
-                for (int q = 0; q < DEC_STAGES; q++) if (q == slot) { fk = kf[q]; fv = vf[q]; }
-                fk *= 64.0f * a.scale_log2e;
-                fv *= 64.0f;
+                const float2 f = *(const float2*)(factors + 2 * at);
+                fk *= 64.0f * f.x;
+                fv = 64.0f * f.y;
             }
             // ---- S = K Q^T: 16 tokens x 8 rows; two chains of products ----
             float sc[NT][4];
@@ -280,7 +274,7 @@ __global__ void __launch_bounds__(DEC_THREADS, DecSmem<D, S8, NT>::CTAS) paged_d
                     for (int c = 0; c < 4; c++) sc[nt][c] = (part[nt][0][c] + part[nt][1][c]) * fk;
             }
             // ---- online softmax (exp2 domain): a lane's tokens are tok0 + g and tok0 + g + 8 ----
-            const bool there = have >> slot & 1;
+            const bool there = have >> at & 1;
             const bool whole = there && tok0 + 15 <= place_lo && (tok0 + 15 < a.sinks || a.window == 0 || tok0 > place_hi - a.window);
             if (!whole) {
 #pragma unroll
@@ -375,6 +369,7 @@ __global__ void __launch_bounds__(DEC_THREADS, DecSmem<D, S8, NT>::CTAS) paged_d
                 do dec_seq(a, ++b, &cur); while (cur.units == 0);
             }
             j1 = (int)min((long long)cur.units, left);
+            slot = 0;
             begin_pair();
             look_up(0);
             for (int j = 0; j < DEC_STAGES - 1; j++) issue(j);
