@@ -79,19 +79,21 @@ __device__ __forceinline__ void load8(const unsigned char* p, float (&x)[8]) {
     }
 }
 
-// The attention of one row (the row-th of sequence b) and query head over blocks [i0, i1) of kb (16 tokens each), by one warp that reads nothing its row does not
-// see: a lane scores one token of 32, then every lane sums D / 32 components of the values.  Into out, or (state given) as a sub-state.  Slow; the
+// The attention of one row (the row-th of sequence b) and query head over blocks [i0, i1) of kb (1 << shift tokens each), by one warp that reads nothing its row does not
+// see: a lane scores one token of 32, then every lane sums D / 32 components of the values.  Into out, or (state given) as a sub-state.  flip: the scale's sign has been
+// taken off it.  Slow; the
 // kernels take it where a value that is no number would reach rows that do not see it through a product of zero.
 template <int D, bool S8>
-__device__ __noinline__ void row_state(const PagedAttn& p, int b, SeqRows s, int row, int head, KeyBlocks kb, int i0, int i1, float* state_o, float* state_ml) {
+__device__ __noinline__ void row_state(const PagedAttn& p, int b, SeqRows s, int row, int head, KeyBlocks kb, int shift, int i0, int i1, float* state_o, float* state_ml,
+                                       unsigned flip) {
     const int lane = threadIdx.x & 31, place = s.len - s.rows + row, hk = head / p.G;
     const unsigned char* q = p.q + (long long)(s.row0 + row) * p.q_rs + (long long)head * p.q_hs;
     constexpr int N = D / 32;
     float acc[N], m = -INFINITY, l = 0.0f;
 #pragma unroll
     for (int e = 0; e < N; e++) acc[e] = 0.0f;
-    for (int i = i0; i < i1; i += 2) {
-        const int block = i + (lane >> 4), tok = key_block(kb, block) * 16 + (lane & 15);
+    for (int x0 = 0; x0 < (i1 - i0) << shift; x0 += 32) {
+        const int x = x0 + lane, block = i0 + (x >> shift), tok = (key_block(kb, block) << shift) + (x & ((1 << shift) - 1));
         int page = -1;
         if (block < i1 && key_visible(tok, place, p.window, p.sinks)) {
             page = table_page(p.c, b, tok >> p.c.page_shift);
@@ -103,12 +105,13 @@ __device__ __noinline__ void row_state(const PagedAttn& p, int b, SeqRows s, int
             float dot = 0.0f;
 #pragma unroll 4
             for (int d = 0; d < D; d += 8) {
-                float k[8], x[8];
+                float k[8], y[8];
                 load8<S8>(p.c.k + at + d * (S8 ? 1 : 2), k);
-                load8<false>(q + 2 * d, x);
+                load8<false>(q + 2 * d, y);
 #pragma unroll
-                for (int e = 0; e < 8; e++) dot = fmaf(x[e], k[e], dot);
+                for (int e = 0; e < 8; e++) dot = fmaf(y[e], k[e], dot);
             }
+            if (flip) dot = -dot;
             if (S8) { dot *= p.c.k_scale[page * p.c.scale_stride + hk]; vs = p.c.v_scale[page * p.c.scale_stride + hk]; }
             score = dot * p.scale_log2e;
         }

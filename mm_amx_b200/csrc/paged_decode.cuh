@@ -434,8 +434,8 @@ __global__ void __launch_bounds__(DEC_THREADS, DecSmem<D, S8, NT>::CTAS) paged_d
         if (odd_value && s.rows > 1) {
             // a value that is no number stands in a block that some rows do not see: row by row, each over what it sees
             for (int i = warp; i < rows; i += DEC_WARPS)
-                row_state<D, S8>(a, at_b, s, i / a.G, at_hk * a.G + i % a.G, kb, 4 * run0, min(4 * run1, kb.count), split ? p.ws_o + (sub + i) * D : nullptr,
-                                 split ? p.ws_ml + (sub + i) * 2 : nullptr);
+                row_state<D, S8>(a, at_b, s, i / a.G, at_hk * a.G + i % a.G, kb, 4, 4 * run0, min(4 * run1, kb.count), split ? p.ws_o + (sub + i) * D : nullptr,
+                                 split ? p.ws_ml + (sub + i) * 2 : nullptr, 0);
         } else if (warp == 0) {
             take_state(st_o + SM::WARP_STATE, 1);
             // through shared memory once more (where warp 0's state would have been), so that rows are stored in whole

@@ -1,0 +1,663 @@
+// Paged attention for more than 16 packed rows (query rows x heads of a group) per sequence and kv head: prompts, chunks of prompts, longer drafts.
+// On the tensor cores (tcgen05), bound by them and by the exponentials beside them.
+//
+// A CTA takes 256 packed rows of one (sequence, kv head), as two tiles of 128 rows, over all 128-token blocks that they see, or over a share of those
+// where the call has too few tiles for the GPU.  Packing the heads of a group into the rows keeps K and V of a block in shared memory for all of them.
+//   warps 0-3, 4-7   softmax of tile 0, 1: a thread has one row.  S comes from tensor memory, exp2(S - max) goes back over it as bf16.  The maximum that is
+//                    subtracted follows the true one only when that is 2^8 ahead (sums and values are fp32 and stay far from their limits, the probabilities'
+//                    rounding is relative), so that O in tensor memory is rescaled hardly ever.
+//   warps 8-11       fetch K and V blocks into a ring of 128-token slots (128-byte swizzle): bf16 by cp.async with zeros for tokens that nobody sees (which
+//                    may hold anything), 8 bits widened on the way to bf16 of (value / 64), exactly; the page's factors go to the softmax.
+//   warp 12          issues the products: S_w = Q_w K^T (Q, K in shared memory), O_w += P_w V (P in tensor memory, V as it lies: N-major).  In the order
+//                    PV_0(j), QK_0(j + 1), PV_1(j), QK_1(j + 1): one tile's products run under the other tile's softmax.
+// Tensor memory: S_0 S_1 (128 columns each; P over the first 64) O_0 O_1 (D columns each).
+// A value that is no number in a block that some rows do not see would reach them as 0 * NaN: the fetching warps look for one in such blocks, and a CTA that
+// met one does its rows again one by one (row_state).
+#pragma once
+#include "paged_common.cuh"
+
+namespace b200fc {
+
+namespace {
+
+constexpr int PR_THREADS = 512;                    // warps 13-15 only fill the fourth group of warps
+constexpr int PR_ROWS = 256, PR_BLOCK = 128;       // packed rows of a CTA, tokens of a block
+constexpr int PR_LOADER = 8, PR_MMA = 12;          // first warps of these roles
+constexpr int PR_META = 8;                         // blocks whose facts are kept; more than the ring holds
+// registers: (SOFTMAX + OTHER) * 256 threads of what the launch has, 128 * 512
+constexpr int PR_REGS_SOFTMAX = 168, PR_REGS_OTHER = 88;
+static_assert((PR_REGS_SOFTMAX + PR_REGS_OTHER) * 256 <= 128 * PR_THREADS, "the split must not ask for more than the launch has");
+
+template <int D> struct PromptSmem {
+    static constexpr int HALF = PR_BLOCK * 128;                       // 128 rows of 64 components
+    static constexpr int TILE = HALF * (D / 64);                      // a tile of Q, a block of K or V
+    static constexpr int SLOTS = D == 128 ? 5 : 8;
+    static constexpr int AHEAD = D == 128 ? 2 : 3;                    // fetched blocks whose arrival is waited for later
+    static constexpr int RING = 2 * TILE, BARS = RING + SLOTS * TILE;
+    static constexpr int META = BARS + 256;
+    static constexpr int BYTES = META + PR_META * 80 + 1024;
+    static_assert(BYTES <= 232448, "shared memory of a CTA");
+};
+struct PromptMeta { unsigned bad; float k[8], v[8]; float pad[3]; };  // of a block: granules of 16 tokens that lie in no page of the pool; factors times 64
+static_assert(sizeof(PromptMeta) == 80, "");
+
+struct PromptParams {
+    PagedAttn a;                  // (scale_log2e: its absolute value, not zero)
+    unsigned flip;                // sign bits of two bf16: the scale's sign, carried by Q
+    int splits;                   // CTAs that share a tile's blocks at most
+    float* ws_o;                  // [CTA][PR_ROWS][D]
+    float* ws_ml;                 // [CTA][PR_ROWS][2]
+    unsigned long long wait_limit_ns;
+};
+
+// operand of which the rows (K dimension, 128 bytes of 64 components each, 128-byte swizzle) lie one behind another: N-major; HALF bytes between 64 components
+__device__ __forceinline__ unsigned long long make_smem_desc_nmajor(unsigned smem_addr, unsigned half) {
+    unsigned long long d = 0;
+    d |= (unsigned long long)((smem_addr & 0x3FFFFu) >> 4);
+    d |= (unsigned long long)(half >> 4) << 16;
+    d |= (unsigned long long)(1024 >> 4) << 32;
+    d |= (unsigned long long)1 << 46;
+    d |= (unsigned long long)2 << 61;
+    return d;
+}
+// instruction descriptor of a 128-row bf16 product with fp32 sums, B K-major or N-major
+__device__ __forceinline__ unsigned make_idesc_bf16(int columns, bool b_nmajor) {
+    return 1u << 4 | 1u << 7 | 1u << 10 | (b_nmajor ? 1u << 16 : 0u) | (unsigned)(columns >> 3) << 17 | (unsigned)(BM >> 4) << 24;
+}
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+__device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// A CTA's work: a tile of a (sequence, kv head) and a share of its blocks.
+struct PromptItem {
+    int b, hk, row0;              // row0: first packed row
+    SeqRows s;
+    KeyBlocks kb;                 // of all its rows, 128 tokens a block
+    int rows;                     // packed rows of the tile
+    int splits, n0, n1;           // shares of the blocks, this one's
+};
+__device__ __forceinline__ int prompt_splits(int count, int splits) { return max(1, min(splits, count >> 1)); }
+// item-th tile: the sequences in order, of each the last rows first (they see most).  By all threads of a block of `threads`.
+template <int THREADS>
+__device__ __forceinline__ bool find_prompt_item(const PagedAttn& a, int item, int split, int splits, bool report, PromptItem* it, int* warp_sum, PromptItem* shared) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    long long seen = 0;
+    bool hit = false;
+    for (int b0 = 0; b0 < a.c.B && !hit; b0 += THREADS) {
+        const int b = b0 + threadIdx.x;
+        SeqRows s{0, 0, 0};
+        if (b < a.c.B && !load_seq(a.c, b, &s) && report) report_paged(a.c);
+        const int packed = s.rows * a.G, tiles = (packed + PR_ROWS - 1) / PR_ROWS, n = tiles * a.c.Hkv;
+        int upto = n;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += u;
+        }
+        __syncthreads();
+        if (lane == 31) warp_sum[warp] = upto;
+        __syncthreads();
+        long long before = 0, all = 0;
+#pragma unroll
+        for (int w = 0; w < THREADS / 32; w++) { before += w < warp ? warp_sum[w] : 0; all += warp_sum[w]; }
+        const long long lo = seen + before + upto - n;
+        if (item >= lo && item < lo + n) {
+            const int at = (int)(item - lo), rt = tiles - 1 - at / a.c.Hkv;
+            PromptItem x;
+            x.b = b; x.hk = at % a.c.Hkv; x.row0 = rt * PR_ROWS; x.s = s;
+            x.rows = min(PR_ROWS, packed - x.row0);
+            const int first = s.len - s.rows;
+            x.kb = key_blocks(max(first + x.row0 / a.G, 0), first + (x.row0 + x.rows - 1) / a.G, a.window, a.sinks, 7);
+            x.splits = prompt_splits(x.kb.count, splits);
+            x.n0 = split < x.splits ? (int)((long long)x.kb.count * split / x.splits) : 0;
+            x.n1 = split < x.splits ? (int)((long long)x.kb.count * (split + 1) / x.splits) : 0;
+            *shared = x;
+        }
+        hit = item >= seen && item < seen + all;
+        seen += all;
+    }
+    __syncthreads();
+    if (hit) *it = *shared;
+    return hit;
+}
+
+template <int D, bool S8>
+__global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const PromptParams p) {
+    using SM = PromptSmem<D>;
+    constexpr int SLOTS = SM::SLOTS, HALF = SM::HALF;
+    extern __shared__ unsigned char pr_smem_raw[];
+    __shared__ int warp_sum[PR_THREADS / 32], odd_value, abort_flag_word;
+    __shared__ unsigned tmem_holder;
+    __shared__ PromptItem item_shared;
+    unsigned char* smem = pr_smem_raw + (((smem_u32(pr_smem_raw) + 1023u) & ~1023u) - smem_u32(pr_smem_raw));
+    unsigned char* ring = smem + SM::RING;
+    const unsigned bars = smem_u32(smem + SM::BARS);
+    const unsigned bar_full = bars, bar_empty = bars + 8 * SLOTS, bar_s = bar_empty + 8 * SLOTS, bar_p = bar_s + 16, bar_o = bar_p + 16, bar_q = bar_o + 8;
+    volatile PromptMeta* meta = (volatile PromptMeta*)(smem + SM::META);
+    volatile int* abort_flag = &abort_flag_word;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const PagedAttn& a = p.a;
+    const unsigned long long limit = p.wait_limit_ns;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < SLOTS; i++) { mbar_init(bar_full + 8 * i, 4); mbar_init(bar_empty + 8 * i, 1); }
+        for (int w = 0; w < 2; w++) { mbar_init(bar_s + 8 * w, 1); mbar_init(bar_p + 8 * w, 4); }
+        mbar_init(bar_o, 1);
+        mbar_init(bar_q, 8);
+        abort_flag_word = 0;
+        odd_value = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == PR_MMA) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_holder)), "r"(512u) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    PromptItem it;
+    const bool has_item = find_prompt_item<PR_THREADS>(a, (int)(blockIdx.x / p.splits), (int)(blockIdx.x % p.splits), p.splits, blockIdx.x == 0, &it, warp_sum, &item_shared);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const unsigned tmem = tmem_holder;
+    const int tiles = has_item ? (it.rows > 128 ? 2 : 1) : 0, n = has_item ? it.n1 - it.n0 : 0;
+    const bool split = has_item && it.splits > 1;
+    const bool work = has_item && (n > 0 || (it.kb.count == 0 && blockIdx.x % p.splits == 0));
+    // places of a tile's first and last row, and which blocks it sees any of
+    const int first_place = has_item ? it.s.len - it.s.rows : 0;
+    auto place_lo = [&](int w) { return first_place + (it.row0 + 128 * w) / a.G; };
+    auto place_hi = [&](int w) { return first_place + (it.row0 + min(128 * w + 127, it.rows - 1)) / a.G; };
+    auto block_token = [&](int j) { return key_block(it.kb, it.n0 + j) << 7; };
+
+    if (warp < PR_LOADER) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PR_REGS_SOFTMAX));
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PR_REGS_OTHER));
+    }
+
+    // (each role ends by itself: behind the branches the roles' numbers of registers would differ)
+    auto all_done = [] { asm volatile("bar.sync 1, %0;" ::"n"(PR_THREADS) : "memory"); };
+    if (warp < PR_LOADER) {
+        if (!work) { all_done(); return; }
+        const int w = warp >> 2, tid = threadIdx.x & 127;
+        if (w < tiles) {
+            // ---- Q tile: rows of 64 components, 128-byte swizzle ----
+            constexpr int CH = D / 8;
+            unsigned char* qt = smem + w * SM::TILE;
+#pragma unroll 4
+            for (int k = 0; k < CH; k++) {
+                const int r = k * (128 / CH) + tid / CH, c = tid % CH, i = it.row0 + 128 * w + r, row = i / a.G;
+                uint4 x = make_uint4(0, 0, 0, 0);
+                if (128 * w + r < it.rows) x = __ldg((const uint4*)(a.q + (long long)(it.s.row0 + row) * a.q_rs + (long long)(it.hk * a.G + i - row * a.G) * a.q_hs) + c);
+                x.x ^= p.flip; x.y ^= p.flip; x.z ^= p.flip; x.w ^= p.flip;
+                *(uint4*)(qt + (c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
+            }
+        }
+        fence_proxy_async();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(bar_q);
+
+        // ---- softmax: a row per thread ----
+        const int i = 128 * w + tid;
+        const bool mine = w < tiles && i < it.rows;
+        const int packed = it.row0 + i, row = packed / a.G, place = first_place + row;
+        const int lo = w < tiles ? place_lo(w) : 0, hi = w < tiles ? place_hi(w) : -1;
+        const unsigned lanes = (unsigned)(warp & 3) << 21;              // lane quarter of tensor memory
+        const unsigned ts = tmem + w * 128 + lanes, to = tmem + 256 + w * D + lanes;
+        const float c = a.scale_log2e;
+        float m_used = -INFINITY, l = 0.0f;
+        unsigned phase = 0;
+        bool alive = true, any = false;
+        for (int j = 0; j < n && w < tiles; j++) {
+            const int tok0 = block_token(j);
+            if (!(tok0 <= hi && (a.window == 0 || tok0 + 127 > lo - a.window || tok0 < a.sinks))) continue;
+            alive = __all_sync(0xffffffffu, mbar_wait(bar_s + 8 * w, phase, abort_flag, limit));
+            if (!alive) break;
+            phase ^= 1;
+            tc_fence_after();
+            const volatile PromptMeta& mt = meta[j % PR_META];
+            const unsigned bad = mt.bad;
+            const bool whole = bad == 0 && tok0 + 127 <= lo && (a.window == 0 || tok0 > hi - a.window || tok0 + 127 < a.sinks);
+            unsigned x[4][32];
+#pragma unroll
+            for (int q = 0; q < 4; q++) tc_ld32(ts + 32 * q, x[q]);
+            tc_wait_ld();
+            if constexpr (S8) {
+#pragma unroll
+                for (int g = 0; g < 8; g++) {
+                    const float f = mt.k[g];
+                    const f32x2 f2 = pack2(f, f);
+#pragma unroll
+                    for (int e = 0; e < 16; e += 2) {
+                        unsigned& u0 = x[g >> 1][(g & 1) * 16 + e];
+                        unsigned& u1 = x[g >> 1][(g & 1) * 16 + e + 1];
+                        float y0, y1;
+                        unpack2(mul2(pack2(__uint_as_float(u0), __uint_as_float(u1)), f2), y0, y1);
+                        u0 = __float_as_uint(y0); u1 = __float_as_uint(y1);
+                    }
+                }
+            }
+            if (!whole) {
+                const int to_hi = place - tok0, from = a.window ? place - a.window - tok0 : -1, sink = min(a.sinks - tok0, 128);
+#pragma unroll
+                for (int e = 0; e < 128; e++) {
+                    const bool seen = e <= to_hi && (e > from || e < sink) && !(bad >> (e >> 4) & 1);
+                    if (!seen) x[e >> 5][e & 31] = 0xff800000u;
+                }
+            }
+            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+            for (int q = 0; q < 4; q++)
+#pragma unroll
+                for (int e = 0; e < 32; e += 8)
+#pragma unroll
+                    for (int u = 0; u < 4; u++) top[u] = max3(top[u], __uint_as_float(x[q][e + 2 * u]), __uint_as_float(x[q][e + 2 * u + 1]));
+            const float m_new = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;      // (c > 0)
+            const bool far = m_new > m_used + 8.0f;
+            if (__any_sync(0xffffffffu, far)) {
+                float f = 1.0f;
+                if (far) { f = exp2_approx(m_used - m_new); m_used = m_new; }
+                l *= f;
+                if (any) {
+                    // (the products into O up to the block before are complete: S of this block was issued behind them)
+#pragma unroll
+                    for (int q = 0; q < D / 32; q++) {
+                        unsigned y[32];
+                        tc_ld32(to + 32 * q, y);
+                        tc_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; e++) y[e] = __float_as_uint(__uint_as_float(y[e]) * f);
+                        tc_st32(to + 32 * q, y);
+                    }
+                }
+            }
+            any = true;
+            const float shift = m_used == -INFINITY ? 0.0f : -m_used;
+            const f32x2 c2 = pack2(c, c), s2 = pack2(shift, shift);
+            f32x2 sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                unsigned pk[32];
+#pragma unroll
+                for (int e = 0; e < 64; e += 2) {
+                    const int g = 4 * h + (e >> 4);
+                    unsigned& u0 = x[2 * h + (e >> 5)][e & 31];
+                    unsigned& u1 = x[2 * h + (e >> 5)][(e & 31) + 1];
+                    float y0, y1;
+                    unpack2(fma2(pack2(__uint_as_float(u0), __uint_as_float(u1)), c2, s2), y0, y1);
+                    y0 = exp2_approx(y0); y1 = exp2_approx(y1);
+                    sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pack2(y0, y1));
+                    if constexpr (S8) {
+                        const float f = mt.v[g];
+                        const float z0 = y0 * f, z1 = y1 * f;
+                        y0 = whole || y0 != 0.0f ? z0 : 0.0f;          // (a masked token has no part in its page's factor, which may be NaN)
+                        y1 = whole || y1 != 0.0f ? z1 : 0.0f;
+                    }
+                    pk[e >> 1] = pack_bf16x2(y0, y1);
+                }
+                tc_st32(ts + 32 * h, pk);
+            }
+            float a0, a1, b0, b1;
+            unpack2(sum[0], a0, a1); unpack2(sum[1], b0, b1);
+            l += (a0 + a1) + (b0 + b1);
+            tc_wait_st();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bar_p + 8 * w);
+        }
+        // ---- O ----
+        if (n > 0 && alive) alive = __all_sync(0xffffffffu, mbar_wait(bar_o, 0, abort_flag, limit));
+        tc_fence_after();
+        if (alive && w < tiles && !*(volatile int*)&odd_value) {
+            const float inv = split ? 1.0f : (l != 0.0f ? 1.0f / l : 0.0f);
+            float* wo = p.ws_o + ((size_t)blockIdx.x * PR_ROWS + i) * D;
+            unsigned char* out = a.out + (long long)(it.s.row0 + row) * a.o_rs + (long long)(it.hk * a.G + packed - row * a.G) * a.o_hs;
+#pragma unroll
+            for (int q = 0; q < D / 32; q++) {
+                unsigned y[32];
+                if (any) {
+                    tc_ld32(to + 32 * q, y);
+                    tc_wait_ld();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e++) y[e] = 0;
+                }
+                if (!mine) continue;
+                if (split) {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 4) *(uint4*)(wo + 32 * q + e) = make_uint4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8) {
+                        unsigned o[4];
+#pragma unroll
+                        for (int u = 0; u < 4; u++) o[u] = pack_bf16x2(__uint_as_float(y[e + 2 * u]) * inv, __uint_as_float(y[e + 2 * u + 1]) * inv);
+                        *(uint4*)(out + (32 * q + e) * 2) = make_uint4(o[0], o[1], o[2], o[3]);
+                    }
+                }
+            }
+            if (split && mine) *(float2*)(p.ws_ml + ((size_t)blockIdx.x * PR_ROWS + i) * 2) = make_float2(m_used, l);
+        }
+        tc_fence_before();
+        all_done();
+        if (odd_value && !abort_flag_word) {
+            for (int r = warp; r < it.rows; r += PR_LOADER) {
+                const int at = it.row0 + r, token = at / a.G;
+                row_state<D, S8>(a, it.b, it.s, token, it.hk * a.G + at - token * a.G, it.kb, 7, it.n0, it.n1,
+                                 split ? p.ws_o + ((size_t)blockIdx.x * PR_ROWS + r) * D : nullptr, split ? p.ws_ml + ((size_t)blockIdx.x * PR_ROWS + r) * 2 : nullptr, p.flip);
+            }
+        }
+    } else if (warp < PR_MMA) {
+        if (!work) { all_done(); return; }
+        // ---- K and V: fill f = 2 j + (0 for K, 1 for V) goes to slot f % SLOTS ----
+        const int tid = threadIdx.x - PR_LOADER * 32;
+        constexpr int CH = S8 ? D / 16 : D / 8, AT_ONCE = 128 / CH, STEPS = 128 / AT_ONCE;    // 16-byte chunks of a token; tokens that the warps take at once
+        const int r0 = tid / CH, ch = tid % CH, psh = a.c.page_shift;
+        const int lo = place_lo(0), hi = place_hi(tiles - 1);
+        int next_page = -1;
+        auto look_up = [&](int j) {                        // lane g < 8: page of granule g of block j
+            next_page = -1;
+            if (j < n && lane < 8) {
+                const int tok = block_token(j) + 16 * lane;
+                if (tok < it.kb.end && (tok + 15 >= it.kb.begin || tok < it.kb.sink_end)) {
+                    next_page = table_page(a.c, it.b, tok >> psh);
+                    if (next_page < 0) report_paged(a.c);
+                }
+            }
+        };
+        auto seen = [&](int tok) { return tok < it.kb.end && (tok >= it.kb.begin || tok < it.kb.sink_end); };
+        bool alive = true;
+        look_up(0);
+        if constexpr (!S8) {
+            auto arrived = [&](int f) {                    // the thread's part of fill f lies in shared memory
+                const int tok0 = block_token(f >> 1);
+                unsigned char* dst = ring + f % SLOTS * SM::TILE;
+                if ((f & 1) && !(tok0 + 127 <= lo && (a.window == 0 || tok0 > hi - a.window || tok0 + 127 < a.sinks))) {
+                    unsigned odd = 0;
+#pragma unroll 4
+                    for (int k = 0; k < STEPS; k++) {
+                        const int r = k * AT_ONCE + r0;
+                        const uint4 x = *(const uint4*)(dst + (ch >> 3) * HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
+                        odd |= not_finite2(x.x) | not_finite2(x.y) | not_finite2(x.z) | not_finite2(x.w);
+                    }
+                    if (odd) odd_value = 1;
+                }
+                fence_proxy_async();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_full + 8 * (f % SLOTS));
+            };
+            for (int j = 0; j < n && alive; j++) {
+                const int tok0 = block_token(j), page = next_page;
+                if (tid < 32) {
+                    const unsigned bad = __ballot_sync(0xffffffffu, lane < 8 && page < 0) & 255u;
+                    if (lane == 0) meta[j % PR_META].bad = bad;
+                }
+                look_up(j + 1);
+#pragma unroll 1
+                for (int kv = 0; kv < 2; kv++) {
+                    const int f = 2 * j + kv, slot = f % SLOTS;
+                    alive = __all_sync(0xffffffffu, mbar_wait(bar_empty + 8 * slot, ((f / SLOTS) & 1) ^ 1, abort_flag, limit));
+                    if (!alive) break;
+                    const unsigned char* base = (kv ? a.c.v : a.c.k) + (long long)it.hk * a.c.head_stride;
+                    const unsigned dst = smem_u32(ring + slot * SM::TILE) + (ch >> 3) * HALF;
+#pragma unroll
+                    for (int k = 0; k < STEPS; k++) {
+                        const int r = k * AT_ONCE + r0, tok = tok0 + r;
+                        const int pg = __shfl_sync(0xffffffffu, page, r >> 4);
+                        const bool ok = pg >= 0 && seen(tok);
+                        const unsigned char* src = base + (ok ? (long long)pg * a.c.page_stride + (long long)(tok & ((1 << psh) - 1)) * a.c.token_stride + ch * 16 : 0);
+                        cp_async16_or_zero(dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4), src, ok);
+                    }
+                    cp_async_commit();
+                    if (f >= SM::AHEAD) { cp_async_wait<SM::AHEAD>(); arrived(f - SM::AHEAD); }
+                }
+            }
+            cp_async_wait<0>();
+            if (alive)
+                for (int f = max(2 * n - SM::AHEAD, 0); f < 2 * n; f++) arrived(f);
+        } else {
+            uint4 data[STEPS];
+            auto fetch = [&](int tok0, int page, int kv) {
+                const unsigned char* base = (kv ? a.c.v : a.c.k) + (long long)it.hk * a.c.head_stride;
+#pragma unroll
+                for (int k = 0; k < STEPS; k++) {
+                    const int r = k * AT_ONCE + r0, tok = tok0 + r;
+                    const int pg = __shfl_sync(0xffffffffu, page, r >> 4);
+                    data[k] = make_uint4(0, 0, 0, 0);
+                    if (pg >= 0 && seen(tok))
+                        data[k] = __ldg((const uint4*)(base + (long long)pg * a.c.page_stride + (long long)(tok & ((1 << psh) - 1)) * a.c.token_stride) + ch);
+                }
+            };
+            int page = next_page;
+            if (n > 0) fetch(block_token(0), page, 0);
+            for (int j = 0; j < n && alive; j++) {
+                if (tid < 32) {
+                    const unsigned bad = __ballot_sync(0xffffffffu, lane < 8 && page < 0) & 255u;
+                    if (lane < 8) {
+                        const long long at = (long long)max(page, 0) * a.c.scale_stride + it.hk;
+                        meta[j % PR_META].k[lane] = page < 0 ? 0.0f : 64.0f * __ldg(a.c.k_scale + at);
+                        meta[j % PR_META].v[lane] = page < 0 ? 0.0f : 64.0f * __ldg(a.c.v_scale + at);
+                    }
+                    if (lane == 0) meta[j % PR_META].bad = bad;
+                }
+                const int tok0 = block_token(j);
+                look_up(j + 1);
+#pragma unroll 1
+                for (int kv = 0; kv < 2; kv++) {
+                    const int f = 2 * j + kv, slot = f % SLOTS;
+                    alive = __all_sync(0xffffffffu, mbar_wait(bar_empty + 8 * slot, ((f / SLOTS) & 1) ^ 1, abort_flag, limit));
+                    if (!alive) break;
+                    unsigned char* dst = ring + slot * SM::TILE;
+#pragma unroll
+                    for (int k = 0; k < STEPS; k++) {
+                        const int r = k * AT_ONCE + r0;
+                        const unsigned q4[4] = {data[k].x, data[k].y, data[k].z, data[k].w};
+                        unsigned o[8];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const unsigned u = q4[e] ^ 0x80808080u;
+                            o[2 * e] = u8x2_to_bf16x2_64th(u, 0x4140);
+                            o[2 * e + 1] = u8x2_to_bf16x2_64th(u, 0x4342);
+                        }
+                        unsigned char* d = dst + (ch >> 2) * HALF + r * 128;
+                        *(uint4*)(d + ((((2 * ch) & 7) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
+                        *(uint4*)(d + ((((2 * ch + 1) & 7) ^ (r & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+                    }
+                    // the next fill's bytes travel while this one is used
+                    if (kv == 0) fetch(tok0, page, 1);
+                    else if (j + 1 < n) { page = next_page; fetch(block_token(j + 1), page, 0); }
+                    fence_proxy_async();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar_full + 8 * slot);
+                }
+            }
+        }
+        all_done();
+    } else if (warp == PR_MMA) {
+        // ---- products ----
+        const unsigned idesc_s = make_idesc_bf16(PR_BLOCK, false), idesc_o = make_idesc_bf16(D, true);
+        int lo[2], hi[2];
+#pragma unroll
+        for (int w = 0; w < 2; w++) { lo[w] = place_lo(w); hi[w] = w < tiles ? place_hi(w) : -1; }
+        auto needed = [&](int w, int j) {
+            if (w >= tiles || j >= n) return false;
+            const int tok0 = block_token(j);
+            return tok0 <= hi[w] && (a.window == 0 || tok0 + 127 > lo[w] - a.window || tok0 < a.sinks);
+        };
+        bool alive = true, begun[2] = {false, false};
+        unsigned p_phase[2] = {0, 0};
+        auto wait = [&](unsigned bar, unsigned parity) {
+            if (alive) alive = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit));
+            tc_fence_after();
+        };
+        auto scores = [&](int w, int j) {
+            const unsigned long long qd = make_smem_desc(smem_u32(smem + w * SM::TILE)), kd = make_smem_desc(smem_u32(ring + (2 * j) % SLOTS * SM::TILE));
+            if (elect_one()) {
+#pragma unroll
+                for (int k = 0; k < D / 16; k++) {
+                    const unsigned long long off = (unsigned long long)((k >> 2) * (HALF >> 4) + (k & 3) * 2);
+                    tc_mma<false>(tmem + w * 128, qd + off, kd + off, idesc_s, (unsigned)(k != 0));
+                }
+                tc_commit(bar_s + 8 * w);
+            }
+            __syncwarp();
+        };
+        if (work && n > 0) {
+            wait(bar_q, 0);
+            wait(bar_full, 0);
+        } else {
+            alive = false;
+        }
+        if (alive) {
+            for (int w = 0; w < 2; w++)
+                if (needed(w, 0)) scores(w, 0);
+            if (elect_one()) tc_commit(bar_empty);
+            __syncwarp();
+        }
+        for (int j = 0; j < n && alive; j++) {
+            const int fv = 2 * j + 1, fk = 2 * j + 2;
+            bool have_v = false, have_k = false;
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                if (needed(w, j)) {
+                    if (!have_v) { wait(bar_full + 8 * (fv % SLOTS), (fv / SLOTS) & 1); have_v = true; }
+                    wait(bar_p + 8 * w, p_phase[w]);
+                    p_phase[w] ^= 1;
+                    if (!alive) break;
+                    const unsigned long long vd = make_smem_desc_nmajor(smem_u32(ring + fv % SLOTS * SM::TILE), HALF);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 0; k < PR_BLOCK / 16; k++)
+                            tc_mma_ts(tmem + 256 + w * D, tmem + w * 128 + k * 8, vd + (unsigned long long)(k * (2048 >> 4)), idesc_o, (unsigned)(begun[w] || k != 0));
+                    }
+                    __syncwarp();
+                    begun[w] = true;
+                }
+                if (needed(w, j + 1)) {
+                    if (!have_k) { wait(bar_full + 8 * (fk % SLOTS), (fk / SLOTS) & 1); have_k = true; }
+                    if (!alive) break;
+                    scores(w, j + 1);
+                }
+            }
+            if (!alive) break;
+            if (elect_one()) {
+                tc_commit(bar_empty + 8 * (fv % SLOTS));
+                if (j + 1 < n) tc_commit(bar_empty + 8 * (fk % SLOTS));
+                else tc_commit(bar_o);
+            }
+            __syncwarp();
+        }
+        asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+        all_done();
+        if (lane == 0 && abort_flag_word) atomicExch(a.c.status, 4);
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+    } else {
+        all_done();
+    }
+}
+
+// Merges the sub-states of tiles whose blocks several CTAs shared: a warp per packed row.
+constexpr int PRC_CTAS = 16;      // CTAs of a tile: 16 rows each
+template <int D>
+__global__ void __launch_bounds__(128) paged_prompt_combine_kernel(const PromptParams p) {
+    __shared__ int warp_sum[4];
+    __shared__ PromptItem item_shared;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const PagedAttn& a = p.a;
+    PromptItem it;
+    if (!find_prompt_item<128>(a, (int)(blockIdx.x / PRC_CTAS), 0, p.splits, false, &it, warp_sum, &item_shared) || it.splits < 2) return;
+    const int lane = threadIdx.x & 31;
+    constexpr int N = D / 32;
+    for (int i = blockIdx.x % PRC_CTAS * 4 + (threadIdx.x >> 5); i < it.rows; i += PRC_CTAS * 4) {
+        const size_t first = ((size_t)(blockIdx.x / PRC_CTAS) * p.splits * PR_ROWS + i);
+        float m = -INFINITY, l = 0.0f, acc[N];
+#pragma unroll
+        for (int e = 0; e < N; e++) acc[e] = 0.0f;
+        for (int q = 0; q < it.splits; q++) {
+            const size_t at = first + (size_t)q * PR_ROWS;
+            const float2 ml = *(const float2*)(p.ws_ml + at * 2);
+            float v[N];
+#pragma unroll
+            for (int e = 0; e < N; e += 2) { const float2 y = *(const float2*)(p.ws_o + at * D + lane * N + e); v[e] = y.x; v[e + 1] = y.y; }
+            const float m_new = fmaxf(m, ml.x), f = m == -INFINITY ? 0.0f : exp2_approx(m - m_new), w = ml.x == -INFINITY ? 0.0f : exp2_approx(ml.x - m_new);
+            l = l * f + ml.y * w;
+#pragma unroll
+            for (int e = 0; e < N; e++) acc[e] = acc[e] * f + v[e] * w;
+            m = m_new;
+        }
+        const int packed = it.row0 + i, row = packed / a.G;
+        unsigned char* out = a.out + (long long)(it.s.row0 + row) * a.o_rs + (long long)(it.hk * a.G + packed - row * a.G) * a.o_hs;
+        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
+        for (int e = 0; e < N; e += 2) *(unsigned*)(out + 2 * (lane * N + e)) = pack2_bf16(acc[e] * inv, acc[e + 1] * inv);
+    }
+}
+
+template <int D, bool S8>
+int launch_paged_prompt(PagedAttn a, float scale, cudaStream_t s) {
+    using SM = PromptSmem<D>;
+    static std::atomic<unsigned long long> attr_devices{0};
+    const int arc = once_per_device(attr_devices, [] {
+        B200FC_CUDA(cudaFuncSetAttribute(paged_prompt_kernel<D, S8>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::BYTES));
+        return (int)B200FC_OK;
+    });
+    if (arc) return arc;
+    PromptParams p;
+    // masked scores are -inf whatever the scale: its sign goes into Q, and zero becomes the smallest number
+    p.flip = scale < 0.0f ? 0x80008000u : 0u;
+    a.scale_log2e = fmaxf(fabsf(a.scale_log2e), FLT_MIN);
+    p.a = a;
+    p.wait_limit_ns = wait_limit_ns();
+    // tiles: full ones, and one more of each sequence
+    const long long bound = ((long long)a.c.T * a.G / PR_ROWS + std::min(a.c.B, a.c.T)) * a.c.Hkv;
+    const long long by_rows = (long long)a.c.B * (((long long)a.c.max_rows * a.G + PR_ROWS - 1) / PR_ROWS) * a.c.Hkv;
+    const long long items = std::min(bound, by_rows);
+    int dev = 0, sms = 148;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    p.splits = (int)std::max(1LL, std::min<long long>(std::min<long long>(16, sms / items), (a.c.capacity / PR_BLOCK + 1) / 2));
+    if (items * p.splits > 0x7fffffffLL / PRC_CTAS) { set_error("paged_attention: too many rows and heads for one call"); return B200FC_ERR_INVALID; }
+    void* ws = nullptr;
+    bool own = false;
+    p.ws_o = p.ws_ml = nullptr;
+    if (p.splits > 1) {
+        const size_t states = (size_t)items * p.splits * PR_ROWS;
+        const int rc = get_stream_scratch(states * (D + 2) * sizeof(float), s, 8, &ws, &own);
+        if (rc) return rc;
+        p.ws_o = (float*)ws;
+        p.ws_ml = p.ws_o + states * D;
+    }
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(items * p.splits));
+    cfg.blockDim = dim3(PR_THREADS);
+    cfg.dynamicSmemBytes = SM::BYTES;
+    cfg.stream = s;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaError_t e = cudaLaunchKernelEx(&cfg, paged_prompt_kernel<D, S8>, (const PromptParams)p);
+    if (e == cudaSuccess) {
+        count_launch();
+        if (p.splits > 1) {
+            cfg.gridDim = dim3((unsigned)(items * PRC_CTAS));
+            cfg.blockDim = dim3(128);
+            cfg.dynamicSmemBytes = 0;
+            e = cudaLaunchKernelEx(&cfg, paged_prompt_combine_kernel<D>, (const PromptParams)p);
+            if (e == cudaSuccess) count_launch();
+        }
+    }
+    if (own) {
+        const cudaError_t f = cudaFreeAsync(ws, s);
+        if (e == cudaSuccess) e = f;
+    }
+    return e == cudaSuccess ? (int)B200FC_OK : cuda_fail(e, "paged prompt attention");
+}
+
+}  // namespace
+
+}  // namespace b200fc
