@@ -6,8 +6,8 @@
 //   warps 0-3, 4-7   softmax of tile 0, 1: a thread has one row.  S comes from tensor memory, exp2(S - max) goes back over it as bf16.  The maximum that is
 //                    subtracted follows the true one only when that is 2^8 ahead (sums and values are fp32 and stay far from their limits, the probabilities'
 //                    rounding is relative), so that O in tensor memory is rescaled hardly ever.
-//   warps 8-11       fetch K and V blocks into a ring of 128-token slots (128-byte swizzle): bf16 by cp.async with zeros for tokens that nobody sees (which
-//                    may hold anything), 8 bits widened on the way to bf16 of (value / 64), exactly; the page's factors go to the softmax.
+//   warps 8-11       fetch K and V blocks into a ring of 128-token slots (128-byte swizzle): bf16 by TMA, or in blocks that not every row sees by cp.async with zeros
+//                    for tokens that nobody sees (which may hold anything), 8 bits widened on the way to bf16 of (value / 64), exactly; the page's factors go to the softmax.
 //   warp 12          issues the products: S_w = Q_w K^T (Q, K in shared memory), O_w += P_w V (P in tensor memory, V as it lies: N-major).  In the order
 //                    PV_0(j), QK_0(j + 1), PV_1(j), QK_1(j + 1): one tile's products run under the other tile's softmax.
 // Tensor memory: S_0 S_1 (128 columns each; P over the first 64) O_0 O_1 (D columns each).
@@ -47,6 +47,7 @@ struct PromptParams {
     int splits;                   // CTAs that share a tile's blocks at most
     float* ws_o;                  // [CTA][PR_ROWS][D]
     float* ws_ml;                 // [CTA][PR_ROWS][2]
+    int tma;                      // the tensor maps are there
     unsigned long long wait_limit_ns;
 };
 
@@ -63,6 +64,19 @@ __device__ __forceinline__ unsigned long long make_smem_desc_nmajor(unsigned sme
 // instruction descriptor of a 128-row bf16 product with fp32 sums, B K-major or N-major
 __device__ __forceinline__ unsigned make_idesc_bf16(int columns, bool b_nmajor) {
     return 1u << 4 | 1u << 7 | 1u << 10 | (b_nmajor ? 1u << 16 : 0u) | (unsigned)(columns >> 3) << 17 | (unsigned)(BM >> 4) << 24;
+}
+__device__ __forceinline__ void tc_st16(unsigned taddr, const unsigned (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+        ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+          "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+__device__ __forceinline__ void tma_load_4d(unsigned dst, const CUtensorMap* map, unsigned bar, int x, int y, int z, int w) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+        ::"r"(dst), "l"(map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+        : "memory");
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
@@ -125,7 +139,7 @@ __device__ __forceinline__ bool find_prompt_item(const PagedAttn& a, int item, i
 }
 
 template <int D, bool S8>
-__global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const PromptParams p) {
+__global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PromptParams p) {
     using SM = PromptSmem<D>;
     constexpr int SLOTS = SM::SLOTS, HALF = SM::HALF;
     extern __shared__ unsigned char pr_smem_raw[];
@@ -263,13 +277,13 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const Promp
                 if (any) {
                     // (the products into O up to the block before are complete: S of this block was issued behind them)
 #pragma unroll
-                    for (int q = 0; q < D / 32; q++) {
-                        unsigned y[32];
-                        tc_ld32(to + 32 * q, y);
+                    for (int q = 0; q < D / 16; q++) {                 // (16 columns at a time: S occupies the registers)
+                        unsigned y[16];
+                        tc_ld16(to + 16 * q, y);
                         tc_wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 32; e++) y[e] = __float_as_uint(__uint_as_float(y[e]) * f);
-                        tc_st32(to + 32 * q, y);
+                        for (int e = 0; e < 16; e++) y[e] = __float_as_uint(__uint_as_float(y[e]) * f);
+                        tc_st16(to + 16 * q, y);
                     }
                 }
             }
@@ -388,35 +402,64 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const Promp
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar_full + 8 * (f % SLOTS));
             };
+            int pending = 0;                               // fills f - pending .. f - 1 are on their way by cp.async
+            const long long ts = a.c.token_stride, thread_off = r0 * ts + ch * 16;
+            const unsigned thread_dst = smem_u32(ring) + (ch >> 3) * HALF + r0 * 128 + (((ch & 7) ^ (r0 & 7)) << 4);
             for (int j = 0; j < n && alive; j++) {
                 const int tok0 = block_token(j), page = next_page;
-                if (tid < 32) {
-                    const unsigned bad = __ballot_sync(0xffffffffu, lane < 8 && page < 0) & 255u;
-                    if (lane == 0) meta[j % PR_META].bad = bad;
-                }
+                const unsigned bad = __ballot_sync(0xffffffffu, lane < 8 && page < 0) & 255u;
+                if (tid == 0) meta[j % PR_META].bad = bad;
                 look_up(j + 1);
+                // blocks that all rows see come by TMA, the others token by token with zeros for those that nobody sees
+                const bool plain = p.tma && bad == 0 && tok0 + 127 <= lo && (a.window == 0 || tok0 > hi - a.window || tok0 + 127 < a.sinks);
 #pragma unroll 1
                 for (int kv = 0; kv < 2; kv++) {
                     const int f = 2 * j + kv, slot = f % SLOTS;
                     alive = __all_sync(0xffffffffu, mbar_wait(bar_empty + 8 * slot, ((f / SLOTS) & 1) ^ 1, abort_flag, limit));
                     if (!alive) break;
-                    const unsigned char* base = (kv ? a.c.v : a.c.k) + (long long)it.hk * a.c.head_stride;
-                    const unsigned dst = smem_u32(ring + slot * SM::TILE) + (ch >> 3) * HALF;
+                    if (plain) {
+                        if (pending) {
+                            cp_async_wait<0>();
+                            for (; pending; pending--) arrived(f - pending);
+                        }
+                        if (warp == PR_LOADER) {
+                            const unsigned full = bar_full + 8 * slot, dst = smem_u32(ring + slot * SM::TILE);
+                            const bool one = elect_one();
+                            if (one) mbar_expect_tx(full, SM::TILE);
+                            const int per = 16 >> (psh - 3);            // pages of a block
 #pragma unroll
-                    for (int k = 0; k < STEPS; k++) {
-                        const int r = k * AT_ONCE + r0, tok = tok0 + r;
-                        const int pg = __shfl_sync(0xffffffffu, page, r >> 4);
-                        const bool ok = pg >= 0 && seen(tok);
-                        const unsigned char* src = base + (ok ? (long long)pg * a.c.page_stride + (long long)(tok & ((1 << psh) - 1)) * a.c.token_stride + ch * 16 : 0);
-                        cp_async16_or_zero(dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4), src, ok);
+                            for (int q = 0; q < 8; q++) {
+                                const int pg = __shfl_sync(0xffffffffu, page, (q << (psh - 4)) & 7);
+                                if (q < per && one) {
+#pragma unroll
+                                    for (int h = 0; h < D / 64; h++) tma_load_4d(dst + h * HALF + (q << (psh + 7)), kv ? &map_v : &map_k, full, 64 * h, 0, it.hk, pg);
+                                }
+                            }
+                            __syncwarp();
+                        } else if (lane == 0) {
+                            mbar_arrive(bar_full + 8 * slot);
+                        }
+                        continue;
+                    }
+                    const unsigned char* base = (kv ? a.c.v : a.c.k) + (long long)it.hk * a.c.head_stride;
+                    const unsigned dst = thread_dst + slot * SM::TILE;
+#pragma unroll
+                    for (int g = 0; g < 8; g++) {
+                        const int pg = __shfl_sync(0xffffffffu, page, g);
+                        const unsigned char* src = base + (long long)max(pg, 0) * a.c.page_stride + ((tok0 + 16 * g) & ((1 << psh) - 1)) * ts + thread_off;
+#pragma unroll
+                        for (int k = 0; k < 16 / AT_ONCE; k++) {
+                            const bool ok = pg >= 0 && seen(tok0 + 16 * g + k * AT_ONCE + r0);
+                            cp_async16_or_zero(dst + (16 * g + k * AT_ONCE) * 128, ok ? src + k * AT_ONCE * ts : base, ok);
+                        }
                     }
                     cp_async_commit();
-                    if (f >= SM::AHEAD) { cp_async_wait<SM::AHEAD>(); arrived(f - SM::AHEAD); }
+                    if (++pending > SM::AHEAD) { cp_async_wait<SM::AHEAD>(); arrived(f - SM::AHEAD); pending--; }
                 }
             }
             cp_async_wait<0>();
             if (alive)
-                for (int f = max(2 * n - SM::AHEAD, 0); f < 2 * n; f++) arrived(f);
+                for (; pending; pending--) arrived(2 * n - pending);
         } else {
             uint4 data[STEPS];
             auto fetch = [&](int tok0, int page, int kv) {
@@ -596,6 +639,20 @@ __global__ void __launch_bounds__(128) paged_prompt_combine_kernel(const PromptP
     }
 }
 
+// A page of one head per box: {64 components, tokens of a page}, 128-byte swizzle.  False where the strides have no tensor map (blocks then come by
+// cp.async, all of them).
+inline bool make_page_map(CUtensorMap* map, const void* base, int D, const PagedView& c) {
+    EncodeTiledFn fn = encode_fn();
+    const uint64_t tokens = 1ull << c.page_shift;
+    const cuuint64_t dims[4] = {(cuuint64_t)D, tokens, (cuuint64_t)c.Hkv, (cuuint64_t)std::max(c.pages, 1)};
+    // (an extent of one is never stepped along)
+    const cuuint64_t strides[3] = {(cuuint64_t)c.token_stride, (cuuint64_t)(c.Hkv > 1 ? c.head_stride : 16), (cuuint64_t)(c.pages > 1 ? c.page_stride : 16)};
+    const cuuint32_t box[4] = {64, (cuuint32_t)tokens, 1, 1}, ones[4] = {1, 1, 1, 1};
+    for (const cuuint64_t st : strides) if (st == 0 || st >= 1ull << 40) return false;
+    return fn && fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, (void*)base, dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int D, bool S8>
 int launch_paged_prompt(PagedAttn a, float scale, cudaStream_t s) {
     using SM = PromptSmem<D>;
@@ -620,6 +677,8 @@ int launch_paged_prompt(PagedAttn a, float scale, cudaStream_t s) {
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     p.splits = (int)std::max(1LL, std::min<long long>(std::min<long long>(16, sms / items), (a.c.capacity / PR_BLOCK + 1) / 2));
     if (items * p.splits > 0x7fffffffLL / PRC_CTAS) { set_error("paged_attention: too many rows and heads for one call"); return B200FC_ERR_INVALID; }
+    CUtensorMap maps[2] = {};
+    p.tma = !S8 && make_page_map(&maps[0], a.c.k, D, a.c) && make_page_map(&maps[1], a.c.v, D, a.c);
     void* ws = nullptr;
     bool own = false;
     p.ws_o = p.ws_ml = nullptr;
@@ -640,7 +699,7 @@ int launch_paged_prompt(PagedAttn a, float scale, cudaStream_t s) {
     cfg.stream = s;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    cudaError_t e = cudaLaunchKernelEx(&cfg, paged_prompt_kernel<D, S8>, (const PromptParams)p);
+    cudaError_t e = cudaLaunchKernelEx(&cfg, paged_prompt_kernel<D, S8>, (const CUtensorMap)maps[0], (const CUtensorMap)maps[1], (const PromptParams)p);
     if (e == cudaSuccess) {
         count_launch();
         if (p.splits > 1) {
