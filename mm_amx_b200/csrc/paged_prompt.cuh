@@ -23,6 +23,7 @@ namespace {
 constexpr int PR_THREADS = 512;                    // warps 13-15 only fill the fourth group of warps
 constexpr int PR_ROWS = 256, PR_BLOCK = 128;       // packed rows of a CTA, tokens of a block
 constexpr int PR_LOADER = 8, PR_MMA = 12;          // first warps of these roles
+constexpr int PR_POLY = 0;                         // of four pairs of exponentials, those by polynomial
 constexpr int PR_META = 8;                         // blocks whose facts are kept; more than the ring holds
 // registers: (SOFTMAX + OTHER) * 256 threads of what the launch has, 128 * 512
 constexpr int PR_REGS_SOFTMAX = 168, PR_REGS_OTHER = 88;
@@ -80,8 +81,29 @@ __device__ __forceinline__ void tma_load_4d(unsigned dst, const CUtensorMap* map
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
+}
+// the lowest n bits, none or all of them beyond 0 .. 32
+__device__ __forceinline__ unsigned first_bits(int n) { return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u); }
+// 2^x for two numbers up to 2^7 without the unit that computes ex2 (16 per clock and SM: it would need as long as the products): x = n + r with
+// |r| <= 1/2 by adding 1.5 * 2^23, 2^r by its minimax polynomial of degree 3 (Remez exchange; relative error 7.5e-5, a twenty-fifth of the rounding to
+// bf16 that follows), n + 100 added to the exponent, and a product with 2^-100 that lets what is below fp32's normal numbers become 0.
+__device__ __forceinline__ f32x2 exp2_poly2(f32x2 x) {
+    const f32x2 magic = pack2(12583012.0f, 12583012.0f), minus = pack2(-12583012.0f, -12583012.0f);      // 1.5 * 2^23 + 100
+    float x0, x1;
+    unpack2(x, x0, x1);
+    x = pack2(fmaxf(x0, -200.0f), fmaxf(x1, -200.0f));
+    const f32x2 t = add2(x, magic), r = fma2(add2(t, minus), pack2(-1.0f, -1.0f), x);
+    f32x2 q = fma2(r, pack2(0.055171669f, 0.055171669f), pack2(0.242611122f, 0.242611122f));
+    q = fma2(q, r, pack2(0.693260985f, 0.693260985f));
+    q = fma2(q, r, pack2(0.999928074f, 0.999928074f));
+    float t0, t1, q0, q1;
+    unpack2(t, t0, t1);
+    unpack2(q, q0, q1);
+    q = pack2(__uint_as_float(__float_as_uint(q0) + (__float_as_uint(t0) << 23)), __uint_as_float(__float_as_uint(q1) + (__float_as_uint(t1) << 23)));
+    asm("mul.rn.ftz.f32x2 %0, %0, %1;" : "+l"(q) : "l"(pack2(0x1p-100f, 0x1p-100f)));
+    return q;
 }
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
@@ -149,7 +171,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
     unsigned char* smem = pr_smem_raw + (((smem_u32(pr_smem_raw) + 1023u) & ~1023u) - smem_u32(pr_smem_raw));
     unsigned char* ring = smem + SM::RING;
     const unsigned bars = smem_u32(smem + SM::BARS);
-    const unsigned bar_full = bars, bar_empty = bars + 8 * SLOTS, bar_s = bar_empty + 8 * SLOTS, bar_p = bar_s + 16, bar_o = bar_p + 16, bar_q = bar_o + 8;
+    const unsigned bar_full = bars, bar_empty = bars + 8 * SLOTS, bar_s = bar_empty + 8 * SLOTS, bar_p = bar_s + 16, bar_o = bar_p + 32, bar_q = bar_o + 8;   // bar_p: [half of the block][tile]
     volatile PromptMeta* meta = (volatile PromptMeta*)(smem + SM::META);
     volatile int* abort_flag = &abort_flag_word;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -158,7 +180,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < SLOTS; i++) { mbar_init(bar_full + 8 * i, 4); mbar_init(bar_empty + 8 * i, 1); }
-        for (int w = 0; w < 2; w++) { mbar_init(bar_s + 8 * w, 1); mbar_init(bar_p + 8 * w, 4); }
+        for (int w = 0; w < 2; w++) { mbar_init(bar_s + 8 * w, 1); mbar_init(bar_p + 8 * w, 4); mbar_init(bar_p + 16 + 8 * w, 4); }
         mbar_init(bar_o, 1);
         mbar_init(bar_q, 8);
         abort_flag_word = 0;
@@ -254,11 +276,15 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
                 }
             }
             if (!whole) {
-                const int to_hi = place - tok0, from = a.window ? place - a.window - tok0 : -1, sink = min(a.sinks - tok0, 128);
+                // bit e of word q: token tok0 + 32 q + e is seen
+                const int to_hi = place - tok0, from = a.window ? place - a.window - tok0 : -1, sink = a.sinks > tok0 ? a.sinks - tok0 : 0;
 #pragma unroll
-                for (int e = 0; e < 128; e++) {
-                    const bool seen = e <= to_hi && (e > from || e < sink) && !(bad >> (e >> 4) & 1);
-                    if (!seen) x[e >> 5][e & 31] = 0xff800000u;
+                for (int q = 0; q < 4; q++) {
+                    unsigned seen = first_bits(to_hi + 1 - 32 * q) & (~first_bits(from + 1 - 32 * q) | first_bits(sink - 32 * q));
+                    if (bad) seen &= ((bad >> (2 * q)) & 1 ? 0u : 0x0000ffffu) | ((bad >> (2 * q + 1)) & 1 ? 0u : 0xffff0000u);
+#pragma unroll
+                    for (int e = 0; e < 32; e++)
+                        if (!(seen & (1u << e))) x[q][e] = 0xff800000u;
                 }
             }
             float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -268,7 +294,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
                 for (int e = 0; e < 32; e += 8)
 #pragma unroll
                     for (int u = 0; u < 4; u++) top[u] = max3(top[u], __uint_as_float(x[q][e + 2 * u]), __uint_as_float(x[q][e + 2 * u + 1]));
-            const float m_new = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * c;      // (c > 0)
+            float m_new = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * c;      // (c > 0)
+            if (!(m_new < INFINITY)) {                                                // an infinity or a NaN among the scores: the row is no number
+                l = __uint_as_float(0x7fc00000u);
+                m_new = m_used;
+            }
             const bool far = m_new > m_used + 8.0f;
             if (__any_sync(0xffffffffu, far)) {
                 float f = 1.0f;
@@ -291,35 +321,45 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
             const float shift = m_used == -INFINITY ? 0.0f : -m_used;
             const f32x2 c2 = pack2(c, c), s2 = pack2(shift, shift);
             f32x2 sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
+            auto half = [&](int h, auto all) {
+                constexpr bool ALL = decltype(all)::value != 0;
                 unsigned pk[32];
 #pragma unroll
                 for (int e = 0; e < 64; e += 2) {
-                    const int g = 4 * h + (e >> 4);
-                    unsigned& u0 = x[2 * h + (e >> 5)][e & 31];
-                    unsigned& u1 = x[2 * h + (e >> 5)][(e & 31) + 1];
+                    const f32x2 y2 = fma2(pack2(__uint_as_float(x[2 * h + (e >> 5)][e & 31]), __uint_as_float(x[2 * h + (e >> 5)][(e & 31) + 1])), c2, s2);
                     float y0, y1;
-                    unpack2(fma2(pack2(__uint_as_float(u0), __uint_as_float(u1)), c2, s2), y0, y1);
-                    y0 = exp2_approx(y0); y1 = exp2_approx(y1);
+                    if (ALL && (e >> 1) % 4 < PR_POLY) {
+                        unpack2(exp2_poly2(y2), y0, y1);
+                    } else {
+                        unpack2(y2, y0, y1);
+                        y0 = exp2_approx(y0); y1 = exp2_approx(y1);
+                    }
                     sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pack2(y0, y1));
                     if constexpr (S8) {
-                        const float f = mt.v[g];
+                        const float f = mt.v[4 * h + (e >> 4)];
                         const float z0 = y0 * f, z1 = y1 * f;
-                        y0 = whole || y0 != 0.0f ? z0 : 0.0f;          // (a masked token has no part in its page's factor, which may be NaN)
-                        y1 = whole || y1 != 0.0f ? z1 : 0.0f;
+                        y0 = ALL || y0 != 0.0f ? z0 : 0.0f;            // (a masked token has no part in its page's factor, which may be NaN)
+                        y1 = ALL || y1 != 0.0f ? z1 : 0.0f;
                     }
                     pk[e >> 1] = pack_bf16x2(y0, y1);
                 }
                 tc_st32(ts + 32 * h, pk);
+                tc_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_p + 16 * h + 8 * w);
+            };
+            // (the first half's product with V runs under the second half's exponentials)
+            if (whole) {
+                half(0, IntConst<1>());
+                half(1, IntConst<1>());
+            } else {
+                half(0, IntConst<0>());
+                half(1, IntConst<0>());
             }
             float a0, a1, b0, b1;
             unpack2(sum[0], a0, a1); unpack2(sum[1], b0, b1);
             l += (a0 + a1) + (b0 + b1);
-            tc_wait_st();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar_p + 8 * w);
         }
         // ---- O ----
         if (n > 0 && alive) alive = __all_sync(0xffffffffu, mbar_wait(bar_o, 0, abort_flag, limit));
@@ -529,69 +569,74 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
             const int tok0 = block_token(j);
             return tok0 <= hi[w] && (a.window == 0 || tok0 + 127 > lo[w] - a.window || tok0 < a.sinks);
         };
-        bool alive = true, begun[2] = {false, false};
-        unsigned p_phase[2] = {0, 0};
-        auto wait = [&](unsigned bar, unsigned parity) {
-            if (alive) alive = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit));
-            tc_fence_after();
-        };
-        auto scores = [&](int w, int j) {
-            const unsigned long long qd = make_smem_desc(smem_u32(smem + w * SM::TILE)), kd = make_smem_desc(smem_u32(ring + (2 * j) % SLOTS * SM::TILE));
+        bool alive = work && n > 0, need[2] = {needed(0, 0), needed(1, 0)}, begun[2] = {false, false};
+        unsigned p_phase[2] = {0, 0}, phase = 0;             // phase: of the ring, at slot `slot`
+        int slot = 0;
+        auto wait = [&](unsigned bar, unsigned parity) { alive = alive && __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit)); };
+        const unsigned long long q_desc = make_smem_desc(smem_u32(smem)), k_desc = make_smem_desc(smem_u32(ring)), v_desc = make_smem_desc_nmajor(smem_u32(ring), HALF);
+        auto scores = [&](int w, int at) {
             if (elect_one()) {
 #pragma unroll
                 for (int k = 0; k < D / 16; k++) {
                     const unsigned long long off = (unsigned long long)((k >> 2) * (HALF >> 4) + (k & 3) * 2);
-                    tc_mma<false>(tmem + w * 128, qd + off, kd + off, idesc_s, (unsigned)(k != 0));
+                    tc_mma<false>(tmem + w * 128, q_desc + (unsigned long long)(w * (SM::TILE >> 4)) + off, k_desc + (unsigned long long)(at * (SM::TILE >> 4)) + off, idesc_s,
+                                  (unsigned)(k != 0));
                 }
                 tc_commit(bar_s + 8 * w);
             }
-            __syncwarp();
         };
-        if (work && n > 0) {
-            wait(bar_q, 0);
-            wait(bar_full, 0);
-        } else {
-            alive = false;
-        }
+        wait(bar_q, 0);
+        wait(bar_full, 0);
         if (alive) {
-            for (int w = 0; w < 2; w++)
-                if (needed(w, 0)) scores(w, 0);
+            tc_fence_after();
+            if (need[0]) scores(0, 0);
+            if (need[1]) scores(1, 0);
             if (elect_one()) tc_commit(bar_empty);
-            __syncwarp();
         }
+        auto advance = [&] { if (++slot == SLOTS) { slot = 0; phase ^= 1; } };
+        advance();
         for (int j = 0; j < n && alive; j++) {
-            const int fv = 2 * j + 1, fk = 2 * j + 2;
-            bool have_v = false, have_k = false;
+            const bool next[2] = {needed(0, j + 1), needed(1, j + 1)};
+            const int vs = slot;
+            const unsigned v_phase = phase;
+            advance();
+            const int ks = slot;
+            const unsigned k_phase = phase;
+            advance();
+            wait(bar_full + 8 * vs, v_phase);
 #pragma unroll
             for (int w = 0; w < 2; w++) {
-                if (needed(w, j)) {
-                    if (!have_v) { wait(bar_full + 8 * (fv % SLOTS), (fv / SLOTS) & 1); have_v = true; }
-                    wait(bar_p + 8 * w, p_phase[w]);
-                    p_phase[w] ^= 1;
-                    if (!alive) break;
-                    const unsigned long long vd = make_smem_desc_nmajor(smem_u32(ring + fv % SLOTS * SM::TILE), HALF);
-                    if (elect_one()) {
+                if (need[w]) {
 #pragma unroll
-                        for (int k = 0; k < PR_BLOCK / 16; k++)
-                            tc_mma_ts(tmem + 256 + w * D, tmem + w * 128 + k * 8, vd + (unsigned long long)(k * (2048 >> 4)), idesc_o, (unsigned)(begun[w] || k != 0));
+                    for (int h = 0; h < 2; h++) {
+                        wait(bar_p + 16 * h + 8 * w, p_phase[w]);
+                        if (!alive) break;
+                        tc_fence_after();
+                        if (elect_one()) {
+#pragma unroll
+                            for (int k = 4 * h; k < 4 * h + 4; k++)
+                                tc_mma_ts(tmem + 256 + w * D, tmem + w * 128 + k * 8, v_desc + (unsigned long long)(vs * (SM::TILE >> 4) + k * (2048 >> 4)), idesc_o,
+                                          (unsigned)(begun[w] || k != 0));
+                        }
                     }
-                    __syncwarp();
+                    p_phase[w] ^= 1;
                     begun[w] = true;
                 }
-                if (needed(w, j + 1)) {
-                    if (!have_k) { wait(bar_full + 8 * (fk % SLOTS), (fk / SLOTS) & 1); have_k = true; }
+                if (next[w]) {
+                    if (w == 0 || !next[0]) wait(bar_full + 8 * ks, k_phase);
                     if (!alive) break;
-                    scores(w, j + 1);
+                    tc_fence_after();
+                    scores(w, ks);
                 }
+                need[w] = next[w];
             }
             if (!alive) break;
             if (elect_one()) {
-                tc_commit(bar_empty + 8 * (fv % SLOTS));
-                if (j + 1 < n) tc_commit(bar_empty + 8 * (fk % SLOTS));
-                else tc_commit(bar_o);
+                tc_commit(bar_empty + 8 * vs);
+                tc_commit(j + 1 < n ? bar_empty + 8 * ks : bar_o);
             }
-            __syncwarp();
         }
+        __syncwarp();
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
         all_done();
         if (lane == 0 && abort_flag_word) atomicExch(a.c.status, 4);
