@@ -8,8 +8,8 @@
 //                    rounding is relative), so that O in tensor memory is rescaled hardly ever.
 //   warps 8-11       fetch K and V blocks into a ring of 128-token slots (128-byte swizzle): bf16 by TMA, or in blocks that not every row sees by cp.async with zeros
 //                    for tokens that nobody sees (which may hold anything), 8 bits widened on the way to bf16 of (value / 64), exactly; the page's factors go to the softmax.
-//   warp 12          issues the products: S_w = Q_w K^T (Q, K in shared memory), O_w += P_w V (P in tensor memory, V as it lies: N-major).  In the order
-//                    PV_0(j), QK_0(j + 1), PV_1(j), QK_1(j + 1): one tile's products run under the other tile's softmax.
+//   warps 12, 13     issue the products of tile 0, 1: S_w = Q_w K^T (Q, K in shared memory), O_w += P_w V (P in tensor memory, V as it lies: N-major).  One
+//                    tile's products run under the other tile's softmax.  (One warp for both tiles was the bottleneck: 3900 clocks a block.)
 // Tensor memory: S_0 S_1 (128 columns each; P over the first 64) O_0 O_1 (D columns each).
 // A value that is no number in a block that some rows do not see would reach them as 0 * NaN: the fetching warps look for one in such blocks, and a CTA that
 // met one does its rows again one by one (row_state).
@@ -20,7 +20,7 @@ namespace b200fc {
 
 namespace {
 
-constexpr int PR_THREADS = 512;                    // warps 13-15 only fill the fourth group of warps
+constexpr int PR_THREADS = 512;                    // warps 14, 15 only fill the fourth group of warps
 constexpr int PR_ROWS = 256, PR_BLOCK = 128;       // packed rows of a CTA, tokens of a block
 constexpr int PR_LOADER = 8, PR_MMA = 12;          // first warps of these roles
 constexpr int PR_POLY = 0;                         // of four pairs of exponentials, those by polynomial
@@ -171,7 +171,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
     unsigned char* smem = pr_smem_raw + (((smem_u32(pr_smem_raw) + 1023u) & ~1023u) - smem_u32(pr_smem_raw));
     unsigned char* ring = smem + SM::RING;
     const unsigned bars = smem_u32(smem + SM::BARS);
-    const unsigned bar_full = bars, bar_empty = bars + 8 * SLOTS, bar_s = bar_empty + 8 * SLOTS, bar_p = bar_s + 16, bar_o = bar_p + 32, bar_q = bar_o + 8;   // bar_p: [half of the block][tile]
+    const unsigned bar_full = bars, bar_empty = bars + 8 * SLOTS, bar_s = bar_empty + 8 * SLOTS, bar_p = bar_s + 16, bar_o = bar_p + 32, bar_q = bar_o + 16;   // bar_p: [half of the block][tile]
     volatile PromptMeta* meta = (volatile PromptMeta*)(smem + SM::META);
     volatile int* abort_flag = &abort_flag_word;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -179,10 +179,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
     const unsigned long long limit = p.wait_limit_ns;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < SLOTS; i++) { mbar_init(bar_full + 8 * i, 4); mbar_init(bar_empty + 8 * i, 1); }
+        for (int i = 0; i < SLOTS; i++) { mbar_init(bar_full + 8 * i, 4); mbar_init(bar_empty + 8 * i, 2); }
         for (int w = 0; w < 2; w++) { mbar_init(bar_s + 8 * w, 1); mbar_init(bar_p + 8 * w, 4); mbar_init(bar_p + 16 + 8 * w, 4); }
-        mbar_init(bar_o, 1);
-        mbar_init(bar_q, 8);
+        for (int w = 0; w < 2; w++) { mbar_init(bar_o + 8 * w, 1); mbar_init(bar_q + 8 * w, 4); }
         abort_flag_word = 0;
         odd_value = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -233,7 +232,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
         }
         fence_proxy_async();
         __syncwarp();
-        if (lane == 0) mbar_arrive(bar_q);
+        if (lane == 0) mbar_arrive(bar_q + 8 * w);
 
         // ---- softmax: a row per thread ----
         const int i = 128 * w + tid;
@@ -362,7 +361,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
             l += (a0 + a1) + (b0 + b1);
         }
         // ---- O ----
-        if (n > 0 && alive) alive = __all_sync(0xffffffffu, mbar_wait(bar_o, 0, abort_flag, limit));
+        if (any && alive) alive = __all_sync(0xffffffffu, mbar_wait(bar_o + 8 * w, 0, abort_flag, limit));
         tc_fence_after();
         if (alive && w < tiles && !*(volatile int*)&odd_value) {
             const float inv = split ? 1.0f : (l != 0.0f ? 1.0f / l : 0.0f);
@@ -558,87 +557,86 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
             }
         }
         all_done();
-    } else if (warp == PR_MMA) {
-        // ---- products ----
+    } else if (warp < PR_MMA + 2) {
+        // ---- products of tile w ----
+        const int w = warp - PR_MMA;
         const unsigned idesc_s = make_idesc_bf16(PR_BLOCK, false), idesc_o = make_idesc_bf16(D, true);
-        int lo[2], hi[2];
-#pragma unroll
-        for (int w = 0; w < 2; w++) { lo[w] = place_lo(w); hi[w] = w < tiles ? place_hi(w) : -1; }
-        auto needed = [&](int w, int j) {
-            if (w >= tiles || j >= n) return false;
+        const int lo = place_lo(w), hi = place_hi(w);
+        auto needed = [&](int j) {
             const int tok0 = block_token(j);
-            return tok0 <= hi[w] && (a.window == 0 || tok0 + 127 > lo[w] - a.window || tok0 < a.sinks);
+            return tok0 <= hi && (a.window == 0 || tok0 + 127 > lo - a.window || tok0 < a.sinks);
         };
-        bool alive = work && n > 0, need[2] = {needed(0, 0), needed(1, 0)}, begun[2] = {false, false};
-        unsigned p_phase[2] = {0, 0}, phase = 0;             // phase: of the ring, at slot `slot`
+        const int frees = tiles == 1 ? 2 : 1;                // arrivals of this tile on a slot's barrier (a lone tile's for both)
+        bool alive = work && n > 0 && w < tiles, begun = false;
+        unsigned p_phase = 0, phase = 0;                     // phase: of the ring, at slot `slot`
         int slot = 0;
+        const unsigned ts = tmem + w * 128, to = tmem + 256 + w * D, bs = bar_s + 8 * w, bp = bar_p + 8 * w;
+        const unsigned long long q_desc = make_smem_desc(smem_u32(smem + w * SM::TILE)), k_desc = make_smem_desc(smem_u32(ring)),
+                                 v_desc = make_smem_desc_nmajor(smem_u32(ring), HALF);
         auto wait = [&](unsigned bar, unsigned parity) { alive = alive && __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit)); };
-        const unsigned long long q_desc = make_smem_desc(smem_u32(smem)), k_desc = make_smem_desc(smem_u32(ring)), v_desc = make_smem_desc_nmajor(smem_u32(ring), HALF);
-        auto scores = [&](int w, int at) {
+        auto free_slot = [&](int at, bool used) {
             if (elect_one()) {
-#pragma unroll
-                for (int k = 0; k < D / 16; k++) {
-                    const unsigned long long off = (unsigned long long)((k >> 2) * (HALF >> 4) + (k & 3) * 2);
-                    tc_mma<false>(tmem + w * 128, q_desc + (unsigned long long)(w * (SM::TILE >> 4)) + off, k_desc + (unsigned long long)(at * (SM::TILE >> 4)) + off, idesc_s,
-                                  (unsigned)(k != 0));
+                for (int i = 0; i < frees; i++) {
+                    if (used) tc_commit(bar_empty + 8 * at);
+                    else mbar_arrive(bar_empty + 8 * at);
                 }
-                tc_commit(bar_s + 8 * w);
             }
         };
-        wait(bar_q, 0);
-        wait(bar_full, 0);
-        if (alive) {
-            tc_fence_after();
-            if (need[0]) scores(0, 0);
-            if (need[1]) scores(1, 0);
-            if (elect_one()) tc_commit(bar_empty);
-        }
-        auto advance = [&] { if (++slot == SLOTS) { slot = 0; phase ^= 1; } };
-        advance();
-        for (int j = 0; j < n && alive; j++) {
-            const bool next[2] = {needed(0, j + 1), needed(1, j + 1)};
-            const int vs = slot;
-            const unsigned v_phase = phase;
-            advance();
-            const int ks = slot;
-            const unsigned k_phase = phase;
-            advance();
-            wait(bar_full + 8 * vs, v_phase);
+        // S of the block whose K is the next fill of the ring
+        auto scores = [&](bool need) {
+            wait(bar_full + 8 * slot, phase);
+            if (!alive) return;
+            if (need) {
+                tc_fence_after();
+                const unsigned long long kd = k_desc + (unsigned long long)(slot * (SM::TILE >> 4));
+                if (elect_one()) {
 #pragma unroll
-            for (int w = 0; w < 2; w++) {
-                if (need[w]) {
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        wait(bar_p + 16 * h + 8 * w, p_phase[w]);
-                        if (!alive) break;
-                        tc_fence_after();
-                        if (elect_one()) {
-#pragma unroll
-                            for (int k = 4 * h; k < 4 * h + 4; k++)
-                                tc_mma_ts(tmem + 256 + w * D, tmem + w * 128 + k * 8, v_desc + (unsigned long long)(vs * (SM::TILE >> 4) + k * (2048 >> 4)), idesc_o,
-                                          (unsigned)(begun[w] || k != 0));
-                        }
+                    for (int k = 0; k < D / 16; k++) {
+                        const unsigned long long off = (unsigned long long)((k >> 2) * (HALF >> 4) + (k & 3) * 2);
+                        tc_mma<false>(ts, q_desc + off, kd + off, idesc_s, (unsigned)(k != 0));
                     }
-                    p_phase[w] ^= 1;
-                    begun[w] = true;
+                    tc_commit(bs);
                 }
-                if (next[w]) {
-                    if (w == 0 || !next[0]) wait(bar_full + 8 * ks, k_phase);
+            }
+            free_slot(slot, need);
+            if (++slot == SLOTS) { slot = 0; phase ^= 1; }
+        };
+        wait(bar_q + 8 * w, 0);
+        bool need = alive && needed(0);
+        if (alive) scores(need);
+        for (int j = 0; j < n && alive; j++) {
+            wait(bar_full + 8 * slot, phase);
+            const int vs = slot;
+            if (++slot == SLOTS) { slot = 0; phase ^= 1; }
+            if (need) {
+                const unsigned long long vd = v_desc + (unsigned long long)(vs * (SM::TILE >> 4));
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    wait(bp + 16 * h, p_phase);
                     if (!alive) break;
                     tc_fence_after();
-                    scores(w, ks);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int k = 4 * h; k < 4 * h + 4; k++) tc_mma_ts(to, ts + k * 8, vd + (unsigned long long)(k * (2048 >> 4)), idesc_o, (unsigned)(begun || k != 0));
+                    }
                 }
-                need[w] = next[w];
+                p_phase ^= 1;
+                begun = true;
             }
             if (!alive) break;
-            if (elect_one()) {
-                tc_commit(bar_empty + 8 * vs);
-                tc_commit(j + 1 < n ? bar_empty + 8 * ks : bar_o);
+            const bool used = need;
+            if (j + 1 < n) {
+                need = needed(j + 1);
+                scores(need);
             }
+            free_slot(vs, used);
         }
+        if (alive && elect_one()) tc_commit(bar_o + 8 * w);
         __syncwarp();
         asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+        tc_fence_before();
         all_done();
+        if (w != 0) return;
         if (lane == 0 && abort_flag_word) atomicExch(a.c.status, 4);
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
