@@ -255,44 +255,58 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
             const volatile PromptMeta& mt = meta[j % PR_META];
             const unsigned bad = mt.bad;
             const bool whole = bad == 0 && tok0 + 127 <= lo && (a.window == 0 || tok0 > hi - a.window || tok0 + 127 < a.sinks);
-            unsigned x[4][32];
-#pragma unroll
-            for (int q = 0; q < 4; q++) tc_ld32(ts + 32 * q, x[q]);
-            tc_wait_ld();
-            if constexpr (S8) {
-#pragma unroll
-                for (int g = 0; g < 8; g++) {
-                    const float f = mt.k[g];
-                    const f32x2 f2 = pack2(f, f);
-#pragma unroll
-                    for (int e = 0; e < 16; e += 2) {
-                        unsigned& u0 = x[g >> 1][(g & 1) * 16 + e];
-                        unsigned& u1 = x[g >> 1][(g & 1) * 16 + e + 1];
-                        float y0, y1;
-                        unpack2(mul2(pack2(__uint_as_float(u0), __uint_as_float(u1)), f2), y0, y1);
-                        u0 = __float_as_uint(y0); u1 = __float_as_uint(y1);
-                    }
-                }
-            }
+            // bit e of seen[q]: token tok0 + 32 q + e is seen
+            unsigned seen[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
             if (!whole) {
-                // bit e of word q: token tok0 + 32 q + e is seen
                 const int to_hi = place - tok0, from = a.window ? place - a.window - tok0 : -1, sink = a.sinks > tok0 ? a.sinks - tok0 : 0;
 #pragma unroll
                 for (int q = 0; q < 4; q++) {
-                    unsigned seen = first_bits(to_hi + 1 - 32 * q) & (~first_bits(from + 1 - 32 * q) | first_bits(sink - 32 * q));
-                    if (bad) seen &= ((bad >> (2 * q)) & 1 ? 0u : 0x0000ffffu) | ((bad >> (2 * q + 1)) & 1 ? 0u : 0xffff0000u);
-#pragma unroll
-                    for (int e = 0; e < 32; e++)
-                        if (!(seen & (1u << e))) x[q][e] = 0xff800000u;
+                    seen[q] = first_bits(to_hi + 1 - 32 * q) & (~first_bits(from + 1 - 32 * q) | first_bits(sink - 32 * q));
+                    seen[q] &= ((bad >> (2 * q)) & 1 ? 0u : 0x0000ffffu) | ((bad >> (2 * q + 1)) & 1 ? 0u : 0xffff0000u);
                 }
             }
+            // ---- the largest score, 32 columns at a time: the next ones are on their way meanwhile ----
+            unsigned xa[32], xb[32];
             float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+            auto largest = [&](unsigned (&x)[32], int q) {
+                if (!whole) {
 #pragma unroll
-            for (int q = 0; q < 4; q++)
+                    for (int e = 0; e < 32; e++)
+                        if (!(seen[q] & (1u << e))) x[e] = 0xff800000u;
+                }
+                if constexpr (S8) {
 #pragma unroll
-                for (int e = 0; e < 32; e += 8)
+                    for (int g = 0; g < 2; g++) {                   // (factors are not negative; none seen stays -inf beside a factor of 0)
+                        float t0 = max3(__uint_as_float(x[16 * g]), __uint_as_float(x[16 * g + 1]), __uint_as_float(x[16 * g + 2]));
+                        float t1 = max3(__uint_as_float(x[16 * g + 3]), __uint_as_float(x[16 * g + 4]), __uint_as_float(x[16 * g + 5]));
 #pragma unroll
-                    for (int u = 0; u < 4; u++) top[u] = max3(top[u], __uint_as_float(x[q][e + 2 * u]), __uint_as_float(x[q][e + 2 * u + 1]));
+                        for (int e = 6; e < 16; e += 4) {
+                            t0 = max3(t0, __uint_as_float(x[16 * g + e]), __uint_as_float(x[16 * g + e + 1]));
+                            if (e + 2 < 16) t1 = max3(t1, __uint_as_float(x[16 * g + e + 2]), __uint_as_float(x[16 * g + e + 3]));
+                        }
+                        t0 = max3(t0, t1, t1);
+                        top[g] = max3(top[g], t0 == -INFINITY ? t0 : t0 * mt.k[2 * q + g], top[g + 2]);
+                    }
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; e += 8)
+#pragma unroll
+                        for (int u = 0; u < 4; u++) top[u] = max3(top[u], __uint_as_float(x[e + 2 * u]), __uint_as_float(x[e + 2 * u + 1]));
+                }
+            };
+            tc_ld32(ts, xa);
+            tc_wait_ld();
+            tc_ld32(ts + 32, xb);
+            largest(xa, 0);
+            tc_wait_ld();
+            tc_ld32(ts + 64, xa);
+            largest(xb, 1);
+            tc_wait_ld();
+            tc_ld32(ts + 96, xb);
+            largest(xa, 2);
+            tc_wait_ld();
+            tc_ld32(ts, xa);
+            largest(xb, 3);
             float m_new = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * c;      // (c > 0)
             if (!(m_new < INFINITY)) {                                                // an infinity or a NaN among the scores: the row is no number
                 l = __uint_as_float(0x7fc00000u);
@@ -306,7 +320,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
                 if (any) {
                     // (the products into O up to the block before are complete: S of this block was issued behind them)
 #pragma unroll
-                    for (int q = 0; q < D / 16; q++) {                 // (16 columns at a time: S occupies the registers)
+                    for (int q = 0; q < D / 16; q++) {
                         unsigned y[16];
                         tc_ld16(to + 16 * q, y);
                         tc_wait_ld();
@@ -320,12 +334,18 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
             const float shift = m_used == -INFINITY ? 0.0f : -m_used;
             const f32x2 c2 = pack2(c, c), s2 = pack2(shift, shift);
             f32x2 sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
-            auto half = [&](int h, auto all) {
+            // ---- probabilities of 32 columns, over the columns of S that have been read ----
+            auto weigh = [&](const unsigned (&x)[32], int q, auto all) {
                 constexpr bool ALL = decltype(all)::value != 0;
-                unsigned pk[32];
+                unsigned pk[16];
 #pragma unroll
-                for (int e = 0; e < 64; e += 2) {
-                    const f32x2 y2 = fma2(pack2(__uint_as_float(x[2 * h + (e >> 5)][e & 31]), __uint_as_float(x[2 * h + (e >> 5)][(e & 31) + 1])), c2, s2);
+                for (int e = 0; e < 32; e += 2) {
+                    f32x2 f2 = c2;
+                    if constexpr (S8) {
+                        const float f = mt.k[2 * q + (e >> 4)] * c;
+                        f2 = pack2(f, f);
+                    }
+                    const f32x2 y2 = fma2(pack2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), f2, s2);
                     float y0, y1;
                     if (ALL && (e >> 1) % 4 < PR_POLY) {
                         unpack2(exp2_poly2(y2), y0, y1);
@@ -333,29 +353,46 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
                         unpack2(y2, y0, y1);
                         y0 = exp2_approx(y0); y1 = exp2_approx(y1);
                     }
+                    if (!ALL) {
+                        if (!(seen[q] & (1u << e))) y0 = 0.0f;
+                        if (!(seen[q] & (2u << e))) y1 = 0.0f;
+                    }
                     sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pack2(y0, y1));
                     if constexpr (S8) {
-                        const float f = mt.v[4 * h + (e >> 4)];
-                        const float z0 = y0 * f, z1 = y1 * f;
-                        y0 = ALL || y0 != 0.0f ? z0 : 0.0f;            // (a masked token has no part in its page's factor, which may be NaN)
-                        y1 = ALL || y1 != 0.0f ? z1 : 0.0f;
+                        const float f = mt.v[2 * q + (e >> 4)];
+                        unpack2(mul2(pack2(y0, y1), pack2(f, f)), y0, y1);
+                        if (!ALL) {                                  // (a masked token has no part in its page's factor, which may be NaN)
+                            if (!(seen[q] & (1u << e))) y0 = 0.0f;
+                            if (!(seen[q] & (2u << e))) y1 = 0.0f;
+                        }
                     }
                     pk[e >> 1] = pack_bf16x2(y0, y1);
                 }
-                tc_st32(ts + 32 * h, pk);
+                tc_st16(ts + 16 * q, pk);
+            };
+            auto hand_over = [&](int h) {
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar_p + 16 * h + 8 * w);
             };
-            // (the first half's product with V runs under the second half's exponentials)
-            if (whole) {
-                half(0, IntConst<1>());
-                half(1, IntConst<1>());
-            } else {
-                half(0, IntConst<0>());
-                half(1, IntConst<0>());
-            }
+            auto all_four = [&](auto all) {
+                tc_wait_ld();
+                tc_ld32(ts + 32, xb);
+                weigh(xa, 0, all);
+                tc_wait_ld();
+                tc_ld32(ts + 64, xa);
+                weigh(xb, 1, all);
+                tc_wait_ld();
+                tc_ld32(ts + 96, xb);
+                weigh(xa, 2, all);
+                hand_over(0);               // (its product with V runs under the last columns' exponentials; waited for here its stores cost nothing)
+                tc_wait_ld();
+                weigh(xb, 3, all);
+                hand_over(1);
+            };
+            if (whole) all_four(IntConst<1>());
+            else all_four(IntConst<0>());
             float a0, a1, b0, b1;
             unpack2(sum[0], a0, a1); unpack2(sum[1], b0, b1);
             l += (a0 + a1) + (b0 + b1);
