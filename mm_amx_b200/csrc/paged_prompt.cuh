@@ -44,6 +44,7 @@ static_assert(sizeof(PromptMeta) == 80, "");
 
 struct PromptParams {
     PagedAttn a;                  // (scale_log2e: its absolute value, not zero)
+    unsigned group_inverse;       // ceil(2^32 / G)
     unsigned flip;                // sign bits of two bf16: the scale's sign, carried by Q
     int splits;                   // CTAs that share a tile's blocks at most
     float* ws_o;                  // [CTA][PR_ROWS][D]
@@ -106,6 +107,13 @@ __device__ __forceinline__ f32x2 exp2_poly2(f32x2 x) {
     return q;
 }
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// n / G for n < 2^31: the product with ceil(2^32 / G) is at most one too large
+__device__ __forceinline__ int over_group(const PromptParams& p, int n) {
+    if (p.a.G == 1) return n;
+    const int q = (int)__umulhi((unsigned)n, p.group_inverse);
+    return q - (q * p.a.G > n);
+}
 
 // A CTA's work: a tile of a (sequence, kv head) and a share of its blocks.
 struct PromptItem {
@@ -202,8 +210,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
     const bool work = has_item && (n > 0 || (it.kb.count == 0 && blockIdx.x % p.splits == 0));
     // places of a tile's first and last row, and which blocks it sees any of
     const int first_place = has_item ? it.s.len - it.s.rows : 0;
-    auto place_lo = [&](int w) { return first_place + (it.row0 + 128 * w) / a.G; };
-    auto place_hi = [&](int w) { return first_place + (it.row0 + min(128 * w + 127, it.rows - 1)) / a.G; };
+    auto place_lo = [&](int w) { return first_place + over_group(p, it.row0 + 128 * w); };
+    auto place_hi = [&](int w) { return first_place + over_group(p, it.row0 + min(128 * w + 127, it.rows - 1)); };
     auto block_token = [&](int j) { return key_block(it.kb, it.n0 + j) << 7; };
 
     if (warp < PR_LOADER) {
@@ -218,16 +226,25 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
         if (!work) { all_done(); return; }
         const int w = warp >> 2, tid = threadIdx.x & 127;
         if (w < tiles) {
-            // ---- Q tile: rows of 64 components, 128-byte swizzle ----
-            constexpr int CH = D / 8;
-            unsigned char* qt = smem + w * SM::TILE;
-#pragma unroll 4
+            // ---- Q tile: rows of 64 components, 128-byte swizzle; zeros behind the last row ----
+            constexpr int CH = D / 8, AT_ONCE = 128 / CH;
+            const int r0 = tid / CH, ch = tid % CH;
+            unsigned char* qt = smem + w * SM::TILE + (ch >> 3) * HALF;
+#pragma unroll
             for (int k = 0; k < CH; k++) {
-                const int r = k * (128 / CH) + tid / CH, c = tid % CH, i = it.row0 + 128 * w + r, row = i / a.G;
-                uint4 x = make_uint4(0, 0, 0, 0);
-                if (128 * w + r < it.rows) x = __ldg((const uint4*)(a.q + (long long)(it.s.row0 + row) * a.q_rs + (long long)(it.hk * a.G + i - row * a.G) * a.q_hs) + c);
-                x.x ^= p.flip; x.y ^= p.flip; x.z ^= p.flip; x.w ^= p.flip;
-                *(uint4*)(qt + (c >> 3) * HALF + r * 128 + (((c & 7) ^ (r & 7)) << 4)) = x;
+                const int r = k * AT_ONCE + r0, i = it.row0 + 128 * w + r, row = over_group(p, i);
+                const bool ok = 128 * w + r < it.rows;
+                cp_async16_or_zero(smem_u32(qt + r * 128 + (((ch & 7) ^ (r & 7)) << 4)),
+                                   ok ? a.q + (long long)(it.s.row0 + row) * a.q_rs + (long long)(it.hk * a.G + i - row * a.G) * a.q_hs + ch * 16 : a.q, ok);
+            }
+            cp_async_commit();
+            cp_async_wait<0>();
+            if (p.flip) {
+                for (int k = 0; k < CH; k++) {
+                    const int r = k * AT_ONCE + r0;
+                    uint4* x = (uint4*)(qt + r * 128 + (((ch & 7) ^ (r & 7)) << 4));
+                    *x = make_uint4(x->x ^ p.flip, x->y ^ p.flip, x->z ^ p.flip, x->w ^ p.flip);
+                }
             }
         }
         fence_proxy_async();
@@ -237,7 +254,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
         // ---- softmax: a row per thread ----
         const int i = 128 * w + tid;
         const bool mine = w < tiles && i < it.rows;
-        const int packed = it.row0 + i, row = packed / a.G, place = first_place + row;
+        const int packed = it.row0 + i, row = over_group(p, packed), place = first_place + row;
         const int lo = w < tiles ? place_lo(w) : 0, hi = w < tiles ? place_hi(w) : -1;
         const unsigned lanes = (unsigned)(warp & 3) << 21;              // lane quarter of tensor memory
         const unsigned ts = tmem + w * 128 + lanes, to = tmem + 256 + w * D + lanes;
@@ -403,7 +420,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
         if (alive && w < tiles && !*(volatile int*)&odd_value) {
             const float inv = split ? 1.0f : (l != 0.0f ? 1.0f / l : 0.0f);
             float* wo = p.ws_o + ((size_t)blockIdx.x * PR_ROWS + i) * D;
-            unsigned char* out = a.out + (long long)(it.s.row0 + row) * a.o_rs + (long long)(it.hk * a.G + packed - row * a.G) * a.o_hs;
+            // rows leave by way of the warp's quarter of the Q tile (all products with it are complete), so that they are stored in whole
+            constexpr int CH = D / 8, AT_ONCE = 32 / CH;
+            unsigned char* own = smem + w * SM::TILE + (warp & 3) * 32 * D * 2;
 #pragma unroll
             for (int q = 0; q < D / 32; q++) {
                 unsigned y[32];
@@ -414,18 +433,28 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
 #pragma unroll
                     for (int e = 0; e < 32; e++) y[e] = 0;
                 }
-                if (!mine) continue;
                 if (split) {
+                    if (mine)
 #pragma unroll
-                    for (int e = 0; e < 32; e += 4) *(uint4*)(wo + 32 * q + e) = make_uint4(y[e], y[e + 1], y[e + 2], y[e + 3]);
+                        for (int e = 0; e < 32; e += 4) *(uint4*)(wo + 32 * q + e) = make_uint4(y[e], y[e + 1], y[e + 2], y[e + 3]);
                 } else {
 #pragma unroll
                     for (int e = 0; e < 32; e += 8) {
                         unsigned o[4];
 #pragma unroll
                         for (int u = 0; u < 4; u++) o[u] = pack_bf16x2(__uint_as_float(y[e + 2 * u]) * inv, __uint_as_float(y[e + 2 * u + 1]) * inv);
-                        *(uint4*)(out + (32 * q + e) * 2) = make_uint4(o[0], o[1], o[2], o[3]);
+                        *(uint4*)(own + lane * D * 2 + (((4 * q + (e >> 3)) ^ (lane & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
                     }
+                }
+            }
+            if (!split) {
+                __syncwarp();
+#pragma unroll
+                for (int k = 0; k < CH; k++) {
+                    const int r = k * AT_ONCE + lane / CH, ch = lane % CH, i2 = 128 * w + (warp & 3) * 32 + r, row2 = over_group(p, it.row0 + i2);
+                    if (i2 < it.rows)
+                        *(uint4*)(a.out + (long long)(it.s.row0 + row2) * a.o_rs + (long long)(it.hk * a.G + it.row0 + i2 - row2 * a.G) * a.o_hs + ch * 16) =
+                            *(const uint4*)(own + r * D * 2 + ((ch ^ (r & 7)) << 4));
                 }
             }
             if (split && mine) *(float2*)(p.ws_ml + ((size_t)blockIdx.x * PR_ROWS + i) * 2) = make_float2(m_used, l);
@@ -743,6 +772,7 @@ int launch_paged_prompt(PagedAttn a, float scale, cudaStream_t s) {
     });
     if (arc) return arc;
     PromptParams p;
+    p.group_inverse = a.G > 1 ? (unsigned)(((1ULL << 32) + a.G - 1) / a.G) : 0;
     // masked scores are -inf whatever the scale: its sign goes into Q, and zero becomes the smallest number
     p.flip = scale < 0.0f ? 0x80008000u : 0u;
     a.scale_log2e = fmaxf(fabsf(a.scale_log2e), FLT_MIN);
