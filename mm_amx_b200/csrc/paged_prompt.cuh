@@ -82,7 +82,7 @@ __device__ __forceinline__ void tma_load_4d(unsigned dst, const CUtensorMap* map
 }
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float r;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
 // the lowest n bits, none or all of them beyond 0 .. 32
@@ -113,6 +113,23 @@ __device__ __forceinline__ int over_group(const PromptParams& p, int n) {
     if (p.a.G == 1) return n;
     const int q = (int)__umulhi((unsigned)n, p.group_inverse);
     return q - (q * p.a.G > n);
+}
+
+// waits, as mbar_wait does, until *word is at least `want`
+__device__ __forceinline__ bool wait_progress(volatile int* word, int want, volatile int* abort_flag, unsigned long long limit) {
+    unsigned long long t0 = 0;
+    while (true) {
+#pragma unroll 1
+        for (int i = 0; i < 64; i++)
+            if (*word >= want) return true;
+        if (*abort_flag) return false;
+        const unsigned long long now = globaltimer();
+        if (t0 == 0) t0 = now;
+        if (now - t0 > limit) {
+            *abort_flag = 1;
+            return false;
+        }
+    }
 }
 
 // A CTA's work: a tile of a (sequence, kv head) and a share of its blocks.
@@ -173,7 +190,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
     using SM = PromptSmem<D>;
     constexpr int SLOTS = SM::SLOTS, HALF = SM::HALF;
     extern __shared__ unsigned char pr_smem_raw[];
-    __shared__ int warp_sum[PR_THREADS / 32], odd_value, abort_flag_word;
+    __shared__ int warp_sum[PR_THREADS / 32], odd_value, abort_flag_word, progress;
     __shared__ unsigned tmem_holder;
     __shared__ PromptItem item_shared;
     unsigned char* smem = pr_smem_raw + (((smem_u32(pr_smem_raw) + 1023u) & ~1023u) - smem_u32(pr_smem_raw));
@@ -192,6 +209,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
         for (int w = 0; w < 2; w++) { mbar_init(bar_o + 8 * w, 1); mbar_init(bar_q + 8 * w, 4); }
         abort_flag_word = 0;
         odd_value = 0;
+        progress = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == PR_MMA) {
@@ -262,9 +280,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
         float m_used = -INFINITY, l = 0.0f;
         unsigned phase = 0;
         bool alive = true, any = false;
+        auto reached = [&](int j) { if (w == 0 && tid == 0) *(volatile int*)&progress = j; };
         for (int j = 0; j < n && w < tiles; j++) {
             const int tok0 = block_token(j);
-            if (!(tok0 <= hi && (a.window == 0 || tok0 + 127 > lo - a.window || tok0 < a.sinks))) continue;
+            if (!(tok0 <= hi && (a.window == 0 || tok0 + 127 > lo - a.window || tok0 < a.sinks))) { reached(j + 1); continue; }
             alive = __all_sync(0xffffffffu, mbar_wait(bar_s + 8 * w, phase, abort_flag, limit));
             if (!alive) break;
             phase ^= 1;
@@ -324,11 +343,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
             tc_wait_ld();
             tc_ld32(ts, xa);
             largest(xb, 3);
-            float m_new = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * c;      // (c > 0)
-            if (!(m_new < INFINITY)) {                                                // an infinity or a NaN among the scores: the row is no number
-                l = __uint_as_float(0x7fc00000u);
-                m_new = m_used;
-            }
+            const float m_new = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * c;      // (c > 0)
             const bool far = m_new > m_used + 8.0f;
             if (__any_sync(0xffffffffu, far)) {
                 float f = 1.0f;
@@ -347,6 +362,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
                     }
                 }
             }
+            /*POINT_B*/
             any = true;
             const float shift = m_used == -INFINITY ? 0.0f : -m_used;
             const f32x2 c2 = pack2(c, c), s2 = pack2(shift, shift);
@@ -400,9 +416,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
                 tc_wait_ld();
                 tc_ld32(ts + 64, xa);
                 weigh(xb, 1, all);
+                /*POINT_C*/
                 tc_wait_ld();
                 tc_ld32(ts + 96, xb);
                 weigh(xa, 2, all);
+                /*POINT_A*/ reached(j + 1);
                 hand_over(0);               // (its product with V runs under the last columns' exponentials; waited for here its stores cost nothing)
                 tc_wait_ld();
                 weigh(xb, 3, all);
@@ -414,6 +432,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
             unpack2(sum[0], a0, a1); unpack2(sum[1], b0, b1);
             l += (a0 + a1) + (b0 + b1);
         }
+        reached(0x7fffffff);
         // ---- O ----
         if (any && alive) alive = __all_sync(0xffffffffu, mbar_wait(bar_o + 8 * w, 0, abort_flag, limit));
         tc_fence_after();
@@ -648,54 +667,66 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
                 }
             }
         };
-        // S of the block whose K is the next fill of the ring
-        auto scores = [&](bool need) {
-            wait(bar_full + 8 * slot, phase);
-            if (!alive) return;
-            if (need) {
-                tc_fence_after();
-                const unsigned long long kd = k_desc + (unsigned long long)(slot * (SM::TILE >> 4));
-                if (elect_one()) {
+        auto step = [&](int& at, unsigned& ph) { if (++at == SLOTS) { at = 0; ph ^= 1; } };
+        auto scores = [&](unsigned long long kd) {           // by one lane
 #pragma unroll
-                    for (int k = 0; k < D / 16; k++) {
-                        const unsigned long long off = (unsigned long long)((k >> 2) * (HALF >> 4) + (k & 3) * 2);
-                        tc_mma<false>(ts, q_desc + off, kd + off, idesc_s, (unsigned)(k != 0));
-                    }
-                    tc_commit(bs);
-                }
+            for (int k = 0; k < D / 16; k++) {
+                const unsigned long long off = (unsigned long long)((k >> 2) * (HALF >> 4) + (k & 3) * 2);
+                tc_mma<false>(ts, q_desc + off, kd + off, idesc_s, (unsigned)(k != 0));
             }
-            free_slot(slot, need);
-            if (++slot == SLOTS) { slot = 0; phase ^= 1; }
+            tc_commit(bs);
+        };
+        auto weighted = [&](unsigned long long vd, int h) {  // by one lane: half of the block's tokens
+#pragma unroll
+            for (int k = 4 * h; k < 4 * h + 4; k++) tc_mma_ts(to, ts + k * 8, vd + (unsigned long long)(k * (2048 >> 4)), idesc_o, (unsigned)(begun || k != 0));
         };
         wait(bar_q + 8 * w, 0);
+        wait(bar_full, 0);
         bool need = alive && needed(0);
-        if (alive) scores(need);
+        if (w == 1 && need) alive = wait_progress(&progress, 1, abort_flag, limit);
+        if (alive) {
+            tc_fence_after();
+            if (need && elect_one()) scores(k_desc);
+            free_slot(0, need);
+            step(slot, phase);
+        }
         for (int j = 0; j < n && alive; j++) {
-            wait(bar_full + 8 * slot, phase);
+            // fills 2 j + 1 (V of this block) and 2 j + 2 (K of the next).  Everything that can be known is known before the last probabilities come:
+            // between them and the next scores there is nothing but products
             const int vs = slot;
-            if (++slot == SLOTS) { slot = 0; phase ^= 1; }
+            wait(bar_full + 8 * slot, phase);
+            step(slot, phase);
+            const unsigned long long vd = v_desc + (unsigned long long)(vs * (SM::TILE >> 4)), kd = k_desc + (unsigned long long)(slot * (SM::TILE >> 4));
+            const bool last = j + 1 == n, next = !last && needed(j + 1);
             if (need) {
-                const unsigned long long vd = v_desc + (unsigned long long)(vs * (SM::TILE >> 4));
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    wait(bp + 16 * h, p_phase);
-                    if (!alive) break;
-                    tc_fence_after();
-                    if (elect_one()) {
-#pragma unroll
-                        for (int k = 4 * h; k < 4 * h + 4; k++) tc_mma_ts(to, ts + k * 8, vd + (unsigned long long)(k * (2048 >> 4)), idesc_o, (unsigned)(begun || k != 0));
-                    }
+                wait(bp, p_phase);
+                if (!alive) break;
+                tc_fence_after();
+                if (elect_one()) weighted(vd, 0);
+            }
+            if (!last) wait(bar_full + 8 * slot, phase);
+            if (w == 1 && next && alive) alive = wait_progress(&progress, j + 2, abort_flag, limit);
+            if (need) {
+                wait(bp + 16, p_phase);
+                if (!alive) break;
+                tc_fence_after();
+                if (elect_one()) {
+                    weighted(vd, 1);
+                    if (next) scores(kd);
                 }
                 p_phase ^= 1;
                 begun = true;
+            } else {
+                if (!alive) break;
+                tc_fence_after();
+                if (next && elect_one()) scores(kd);
             }
-            if (!alive) break;
-            const bool used = need;
-            if (j + 1 < n) {
-                need = needed(j + 1);
-                scores(need);
+            free_slot(vs, need);
+            if (!last) {
+                free_slot(slot, next);
+                step(slot, phase);
             }
-            free_slot(vs, used);
+            need = next;
         }
         if (alive && elect_one()) tc_commit(bar_o + 8 * w);
         __syncwarp();
