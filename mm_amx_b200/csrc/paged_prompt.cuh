@@ -115,23 +115,6 @@ __device__ __forceinline__ int over_group(const PromptParams& p, int n) {
     return q - (q * p.a.G > n);
 }
 
-// waits, as mbar_wait does, until *word is at least `want`
-__device__ __forceinline__ bool wait_progress(volatile int* word, int want, volatile int* abort_flag, unsigned long long limit) {
-    unsigned long long t0 = 0;
-    while (true) {
-#pragma unroll 1
-        for (int i = 0; i < 64; i++)
-            if (*word >= want) return true;
-        if (*abort_flag) return false;
-        const unsigned long long now = globaltimer();
-        if (t0 == 0) t0 = now;
-        if (now - t0 > limit) {
-            *abort_flag = 1;
-            return false;
-        }
-    }
-}
-
 // A CTA's work: a tile of a (sequence, kv head) and a share of its blocks.
 struct PromptItem {
     int b, hk, row0;              // row0: first packed row
@@ -190,13 +173,13 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
     using SM = PromptSmem<D>;
     constexpr int SLOTS = SM::SLOTS, HALF = SM::HALF;
     extern __shared__ unsigned char pr_smem_raw[];
-    __shared__ int warp_sum[PR_THREADS / 32], odd_value, abort_flag_word, progress;
+    __shared__ int warp_sum[PR_THREADS / 32], odd_value, abort_flag_word;
     __shared__ unsigned tmem_holder;
     __shared__ PromptItem item_shared;
     unsigned char* smem = pr_smem_raw + (((smem_u32(pr_smem_raw) + 1023u) & ~1023u) - smem_u32(pr_smem_raw));
     unsigned char* ring = smem + SM::RING;
     const unsigned bars = smem_u32(smem + SM::BARS);
-    const unsigned bar_full = bars, bar_empty = bars + 8 * SLOTS, bar_s = bar_empty + 8 * SLOTS, bar_p = bar_s + 16, bar_o = bar_p + 32, bar_q = bar_o + 16;   // bar_p: [half of the block][tile]
+    const unsigned bar_full = bars, bar_empty = bars + 8 * SLOTS, bar_s = bar_empty + 8 * SLOTS, bar_p = bar_s + 16, bar_o = bar_p + 32, bar_q = bar_o + 16, bar_turn = bar_q + 16;   // bar_p: [half of the block][tile]
     volatile PromptMeta* meta = (volatile PromptMeta*)(smem + SM::META);
     volatile int* abort_flag = &abort_flag_word;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -206,10 +189,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
     if (threadIdx.x == 0) {
         for (int i = 0; i < SLOTS; i++) { mbar_init(bar_full + 8 * i, 4); mbar_init(bar_empty + 8 * i, 2); }
         for (int w = 0; w < 2; w++) { mbar_init(bar_s + 8 * w, 1); mbar_init(bar_p + 8 * w, 4); mbar_init(bar_p + 16 + 8 * w, 4); }
-        for (int w = 0; w < 2; w++) { mbar_init(bar_o + 8 * w, 1); mbar_init(bar_q + 8 * w, 4); }
+        for (int w = 0; w < 2; w++) { mbar_init(bar_o + 8 * w, 1); mbar_init(bar_q + 8 * w, 4); mbar_init(bar_turn + 8 * w, 4); }
         abort_flag_word = 0;
         odd_value = 0;
-        progress = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == PR_MMA) {
@@ -280,10 +262,24 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
         float m_used = -INFINITY, l = 0.0f;
         unsigned phase = 0;
         bool alive = true, any = false;
-        auto reached = [&](int j) { if (w == 0 && tid == 0) *(volatile int*)&progress = j; };
+        // The two tiles take their exponentials in turns (tile 0, tile 1, tile 0, ...): side by side each would wait for the other's, and then both for their
+        // products.  One turn for each block, seen or not.
+        auto take_turn = [&](int j) {
+            if (tiles == 2 && (w == 1 || j > 0)) alive = alive && __all_sync(0xffffffffu, mbar_wait(bar_turn + 8 * w, (unsigned)(w == 1 ? j : j - 1) & 1, abort_flag, limit));
+        };
+        auto pass_turn = [&] {
+            if (tiles == 2) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_turn + 8 * (1 - w));
+            }
+        };
         for (int j = 0; j < n && w < tiles; j++) {
             const int tok0 = block_token(j);
-            if (!(tok0 <= hi && (a.window == 0 || tok0 + 127 > lo - a.window || tok0 < a.sinks))) { reached(j + 1); continue; }
+            if (!(tok0 <= hi && (a.window == 0 || tok0 + 127 > lo - a.window || tok0 < a.sinks))) {
+                take_turn(j);
+                pass_turn();
+                continue;
+            }
             alive = __all_sync(0xffffffffu, mbar_wait(bar_s + 8 * w, phase, abort_flag, limit));
             if (!alive) break;
             phase ^= 1;
@@ -362,7 +358,6 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
                     }
                 }
             }
-            /*POINT_B*/
             any = true;
             const float shift = m_used == -INFINITY ? 0.0f : -m_used;
             const f32x2 c2 = pack2(c, c), s2 = pack2(shift, shift);
@@ -409,6 +404,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar_p + 16 * h + 8 * w);
             };
+            take_turn(j);
+            if (!alive) break;
             auto all_four = [&](auto all) {
                 tc_wait_ld();
                 tc_ld32(ts + 32, xb);
@@ -416,14 +413,13 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
                 tc_wait_ld();
                 tc_ld32(ts + 64, xa);
                 weigh(xb, 1, all);
-                /*POINT_C*/
                 tc_wait_ld();
                 tc_ld32(ts + 96, xb);
                 weigh(xa, 2, all);
-                /*POINT_A*/ reached(j + 1);
                 hand_over(0);               // (its product with V runs under the last columns' exponentials; waited for here its stores cost nothing)
                 tc_wait_ld();
                 weigh(xb, 3, all);
+                pass_turn();
                 hand_over(1);
             };
             if (whole) all_four(IntConst<1>());
@@ -432,7 +428,6 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
             unpack2(sum[0], a0, a1); unpack2(sum[1], b0, b1);
             l += (a0 + a1) + (b0 + b1);
         }
-        reached(0x7fffffff);
         // ---- O ----
         if (any && alive) alive = __all_sync(0xffffffffu, mbar_wait(bar_o + 8 * w, 0, abort_flag, limit));
         tc_fence_after();
@@ -683,7 +678,6 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
         wait(bar_q + 8 * w, 0);
         wait(bar_full, 0);
         bool need = alive && needed(0);
-        if (w == 1 && need) alive = wait_progress(&progress, 1, abort_flag, limit);
         if (alive) {
             tc_fence_after();
             if (need && elect_one()) scores(k_desc);
@@ -705,7 +699,6 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
                 if (elect_one()) weighted(vd, 0);
             }
             if (!last) wait(bar_full + 8 * slot, phase);
-            if (w == 1 && next && alive) alive = wait_progress(&progress, j + 2, abort_flag, limit);
             if (need) {
                 wait(bp + 16, p_phase);
                 if (!alive) break;
