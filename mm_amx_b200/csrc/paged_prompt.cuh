@@ -124,46 +124,83 @@ struct PromptItem {
     int splits, n0, n1;           // shares of the blocks, this one's
 };
 __device__ __forceinline__ int prompt_splits(int count, int splits) { return max(1, min(splits, count >> 1)); }
-// item-th tile: the sequences in order, of each the last rows first (they see most).  By all threads of a block of `threads`.
+// item-th tile: of each sequence the last rows first (they see most), and of up to PR_RANKED sequences those whose last tile sees most first, so that no long
+// tile is left for the end (3 sequences of up to 2048 rows and 4096 tokens: 209 us in the order given, 193 so).  By all threads of a block.
+constexpr int PR_RANKED = 64;
 template <int THREADS>
 __device__ __forceinline__ bool find_prompt_item(const PagedAttn& a, int item, int split, int splits, bool report, PromptItem* it, int* warp_sum, PromptItem* shared) {
+    __shared__ int keys[PR_RANKED], order[PR_RANKED];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    long long seen = 0;
-    bool hit = false;
-    for (int b0 = 0; b0 < a.c.B && !hit; b0 += THREADS) {
-        const int b = b0 + threadIdx.x;
-        SeqRows s{0, 0, 0};
-        if (b < a.c.B && !load_seq(a.c, b, &s) && report) report_paged(a.c);
-        const int packed = s.rows * a.G, tiles = (packed + PR_ROWS - 1) / PR_ROWS, n = tiles * a.c.Hkv;
-        int upto = n;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int u = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += u;
+    auto sequence = [&](int b, SeqRows* s, int* tiles) {
+        *s = SeqRows{0, 0, 0};
+        const bool ok = load_seq(a.c, b, s);
+        *tiles = (s->rows * a.G + PR_ROWS - 1) / PR_ROWS;
+        return ok;
+    };
+    auto found = [&](int b, const SeqRows& s, int tiles, int at) {
+        const int rt = tiles - 1 - at / a.c.Hkv, first = s.len - s.rows;
+        PromptItem x;
+        x.b = b; x.hk = at % a.c.Hkv; x.row0 = rt * PR_ROWS; x.s = s;
+        x.rows = min(PR_ROWS, s.rows * a.G - x.row0);
+        x.kb = key_blocks(max(first + x.row0 / a.G, 0), first + (x.row0 + x.rows - 1) / a.G, a.window, a.sinks, 7);
+        x.splits = prompt_splits(x.kb.count, splits);
+        x.n0 = split < x.splits ? (int)((long long)x.kb.count * split / x.splits) : 0;
+        x.n1 = split < x.splits ? (int)((long long)x.kb.count * (split + 1) / x.splits) : 0;
+        *shared = x;
+    };
+    if (threadIdx.x == 0) shared->b = -1;
+    if (a.c.B <= PR_RANKED) {
+        const int b = threadIdx.x;
+        SeqRows s;
+        int tiles = 0, key = 0, n = 0;
+        if (b < a.c.B) {
+            if (!sequence(b, &s, &tiles) && report) report_paged(a.c);
+            n = tiles * a.c.Hkv;
+            const KeyBlocks kb = key_blocks(max(s.len - 1 - (PR_ROWS - 1) / a.G, 0), s.len - 1, a.window, a.sinks, 7);
+            key = n ? kb.count : -1;
+            keys[b] = key;
         }
         __syncthreads();
-        if (lane == 31) warp_sum[warp] = upto;
-        __syncthreads();
-        long long before = 0, all = 0;
-#pragma unroll
-        for (int w = 0; w < THREADS / 32; w++) { before += w < warp ? warp_sum[w] : 0; all += warp_sum[w]; }
-        const long long lo = seen + before + upto - n;
-        if (item >= lo && item < lo + n) {
-            const int at = (int)(item - lo), rt = tiles - 1 - at / a.c.Hkv;
-            PromptItem x;
-            x.b = b; x.hk = at % a.c.Hkv; x.row0 = rt * PR_ROWS; x.s = s;
-            x.rows = min(PR_ROWS, packed - x.row0);
-            const int first = s.len - s.rows;
-            x.kb = key_blocks(max(first + x.row0 / a.G, 0), first + (x.row0 + x.rows - 1) / a.G, a.window, a.sinks, 7);
-            x.splits = prompt_splits(x.kb.count, splits);
-            x.n0 = split < x.splits ? (int)((long long)x.kb.count * split / x.splits) : 0;
-            x.n1 = split < x.splits ? (int)((long long)x.kb.count * (split + 1) / x.splits) : 0;
-            *shared = x;
+        if (b < a.c.B) {
+            int rank = 0;
+            for (int o = 0; o < a.c.B; o++) rank += keys[o] > key || (keys[o] == key && o < b);
+            order[rank] = n;
+            n = rank;                                        // (from here on the sequence's place in the order)
         }
-        hit = item >= seen && item < seen + all;
-        seen += all;
+        __syncthreads();
+        if (b < a.c.B && tiles) {
+            int before = 0;
+            for (int o = 0; o < n; o++) before += order[o];
+            if (item >= before && item < before + tiles * a.c.Hkv) found(b, s, tiles, item - before);
+        }
+        __syncthreads();
+    } else {
+        long long seen = 0;
+        for (int b0 = 0; b0 < a.c.B && seen <= item; b0 += THREADS) {
+            const int b = b0 + threadIdx.x;
+            SeqRows s;
+            int tiles = 0;
+            if (b < a.c.B && !sequence(b, &s, &tiles) && report) report_paged(a.c);
+            const int n = tiles * a.c.Hkv;
+            int upto = n;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += u;
+            }
+            __syncthreads();
+            if (lane == 31) warp_sum[warp] = upto;
+            __syncthreads();
+            long long before = 0, all = 0;
+#pragma unroll
+            for (int w = 0; w < THREADS / 32; w++) { before += w < warp ? warp_sum[w] : 0; all += warp_sum[w]; }
+            const long long lo = seen + before + upto - n;
+            if (item >= lo && item < lo + n) found(b, s, tiles, (int)(item - lo));
+            seen += all;
+        }
+        __syncthreads();
     }
-    __syncthreads();
+    const bool hit = shared->b >= 0;
     if (hit) *it = *shared;
     return hit;
 }
