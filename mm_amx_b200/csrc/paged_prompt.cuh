@@ -3,14 +3,14 @@
 //
 // A CTA takes 256 packed rows of one (sequence, kv head), as two tiles of 128 rows, over all 128-token blocks that they see, or over a share of those
 // where the call has too few tiles for the GPU.  Packing the heads of a group into the rows keeps K and V of a block in shared memory for all of them.
-//   warps 0-3, 4-7   softmax of tile 0, 1: a thread has one row.  S comes from tensor memory, exp2(S - max) goes back over it as bf16.  The maximum that is
-//                    subtracted follows the true one only when that is 2^8 ahead (sums and values are fp32 and stay far from their limits, the probabilities'
-//                    rounding is relative), so that O in tensor memory is rescaled hardly ever.
+//   warps 0-3, 4-7   softmax of tile 0, 1: a thread has one row.  S comes from tensor memory 64 tokens at a time, exp2(S - max) goes back over it as bf16.  The
+//                    maximum that is subtracted follows the true one only when that is 2^8 ahead (sums and values are fp32 and stay far from their limits, the
+//                    probabilities' rounding is relative), so that O in tensor memory is rescaled hardly ever.
 //   warps 8-11       fetch K and V blocks into a ring of 128-token slots (128-byte swizzle): bf16 by TMA, or in blocks that not every row sees by cp.async with zeros
 //                    for tokens that nobody sees (which may hold anything), 8 bits widened on the way to bf16 of (value / 64), exactly; the page's factors go to the softmax.
 //   warps 12, 13     issue the products of tile 0, 1: S_w = Q_w K^T (Q, K in shared memory), O_w += P_w V (P in tensor memory, V as it lies: N-major).  One
 //                    tile's products run under the other tile's softmax.  (One warp for both tiles was the bottleneck: 3900 clocks a block.)
-// Tensor memory: S_0 S_1 (128 columns each; P over the first 64) O_0 O_1 (D columns each).
+// Tensor memory: S_0 S_1 (128 columns each; P over the first half of either 64) O_0 O_1 (D columns each).
 // A value that is no number in a block that some rows do not see would reach them as 0 * NaN: the fetching warps look for one in such blocks, and a CTA that
 // met one does its rows again one by one (row_state).
 #pragma once
@@ -20,14 +20,11 @@ namespace b200fc {
 
 namespace {
 
-constexpr int PR_THREADS = 512;                    // warps 14, 15 only fill the fourth group of warps
+constexpr int PR_THREADS = 448;
 constexpr int PR_ROWS = 256, PR_BLOCK = 128;       // packed rows of a CTA, tokens of a block
-constexpr int PR_LOADER = 8, PR_MMA = 12;          // first warps of these roles
+constexpr int PR_LOADER = 8, PR_MMA = 12;          // first warps of these roles (the last one does nothing else)
 constexpr int PR_POLY = 0;                         // of four pairs of exponentials, those by polynomial
 constexpr int PR_META = 8;                         // blocks whose facts are kept; more than the ring holds
-// registers: (SOFTMAX + OTHER) * 256 threads of what the launch has, 128 * 512
-constexpr int PR_REGS_SOFTMAX = 168, PR_REGS_OTHER = 88;
-static_assert((PR_REGS_SOFTMAX + PR_REGS_OTHER) * 256 <= 128 * PR_THREADS, "the split must not ask for more than the launch has");
 
 template <int D> struct PromptSmem {
     static constexpr int HALF = PR_BLOCK * 128;                       // 128 rows of 64 components
@@ -35,8 +32,9 @@ template <int D> struct PromptSmem {
     static constexpr int SLOTS = D == 128 ? 5 : 8;
     static constexpr int AHEAD = D == 128 ? 2 : 3;                    // fetched blocks whose arrival is waited for later
     static constexpr int RING = 2 * TILE, BARS = RING + SLOTS * TILE;
-    static constexpr int META = BARS + 256;
-    static constexpr int BYTES = META + PR_META * 80 + 1024;
+    static constexpr int META = BARS + 384;
+    static constexpr int ROWS = META + PR_META * 80;                  // what a row's two threads tell one another; before that, the search for the tile
+    static constexpr int BYTES = ROWS + 2 * 128 * 2 * 4;              // (D = 128: all there is)
     static_assert(BYTES <= 232448, "shared memory of a CTA");
 };
 struct PromptMeta { unsigned bad; float k[8], v[8]; float pad[3]; };  // of a block: granules of 16 tokens that lie in no page of the pool; factors times 64
@@ -127,9 +125,15 @@ __device__ __forceinline__ int prompt_splits(int count, int splits) { return max
 // item-th tile: of each sequence the last rows first (they see most), and of up to PR_RANKED sequences those whose last tile sees most first, so that no long
 // tile is left for the end (3 sequences of up to 2048 rows and 4096 tokens: 209 us in the order given, 193 so).  By all threads of a block.
 constexpr int PR_RANKED = 64;
+struct FindSpace {
+    PromptItem item;
+    int warp_sum[PR_THREADS / 32], keys[PR_RANKED], order[PR_RANKED];
+};
+static_assert(sizeof(FindSpace) <= 2048, "lies where the rows' values come later");
 template <int THREADS>
-__device__ __forceinline__ bool find_prompt_item(const PagedAttn& a, int item, int split, int splits, bool report, PromptItem* it, int* warp_sum, PromptItem* shared) {
-    __shared__ int keys[PR_RANKED], order[PR_RANKED];
+__device__ __forceinline__ bool find_prompt_item(const PagedAttn& a, int item, int split, int splits, bool report, PromptItem* it, FindSpace* space) {
+    PromptItem* shared = &space->item;
+    int *warp_sum = space->warp_sum, *keys = space->keys, *order = space->order;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     auto sequence = [&](int b, SeqRows* s, int* tiles) {
         *s = SeqRows{0, 0, 0};
@@ -169,9 +173,9 @@ __device__ __forceinline__ bool find_prompt_item(const PagedAttn& a, int item, i
         }
         __syncthreads();
         if (b < a.c.B && tiles) {
-            int before = 0;
+            long long before = 0;
             for (int o = 0; o < n; o++) before += order[o];
-            if (item >= before && item < before + tiles * a.c.Hkv) found(b, s, tiles, item - before);
+            if (item >= before && item < before + tiles * a.c.Hkv) found(b, s, tiles, (int)(item - before));
         }
         __syncthreads();
     } else {
@@ -209,14 +213,19 @@ template <int D, bool S8>
 __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PromptParams p) {
     using SM = PromptSmem<D>;
     constexpr int SLOTS = SM::SLOTS, HALF = SM::HALF;
-    extern __shared__ unsigned char pr_smem_raw[];
-    __shared__ int warp_sum[PR_THREADS / 32], odd_value, abort_flag_word;
-    __shared__ unsigned tmem_holder;
-    __shared__ PromptItem item_shared;
-    unsigned char* smem = pr_smem_raw + (((smem_u32(pr_smem_raw) + 1023u) & ~1023u) - smem_u32(pr_smem_raw));
+    // no static shared memory: the dynamic part then begins at a multiple of 1024, as the swizzle wants it
+    extern __shared__ __align__(1024) unsigned char smem[];
+    int& odd_value = *(int*)(smem + SM::BARS + 368);
+    int& abort_flag_word = *(int*)(smem + SM::BARS + 372);
+    unsigned& tmem_holder = *(unsigned*)(smem + SM::BARS + 376);
+    float* row_values = (float*)(smem + SM::ROWS);
+    if (smem_u32(smem) & 1023u) {
+        if (threadIdx.x == 0) atomicExch(p.a.c.status, 4);
+        return;
+    }
     unsigned char* ring = smem + SM::RING;
     const unsigned bars = smem_u32(smem + SM::BARS);
-    const unsigned bar_full = bars, bar_empty = bars + 8 * SLOTS, bar_s = bar_empty + 8 * SLOTS, bar_p = bar_s + 16, bar_o = bar_p + 32, bar_q = bar_o + 16, bar_turn = bar_q + 16;   // bar_p: [half of the block][tile]
+    const unsigned bar_full = bars, bar_empty = bars + 8 * SLOTS, bar_s = bar_empty + 8 * SLOTS, bar_p = bar_s + 32, bar_v = bar_p + 32, bar_o = bar_v + 16, bar_q = bar_o + 16;   // bar_s, bar_p: [half of the block][tile]
     volatile PromptMeta* meta = (volatile PromptMeta*)(smem + SM::META);
     volatile int* abort_flag = &abort_flag_word;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -225,8 +234,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < SLOTS; i++) { mbar_init(bar_full + 8 * i, 4); mbar_init(bar_empty + 8 * i, 2); }
-        for (int w = 0; w < 2; w++) { mbar_init(bar_s + 8 * w, 1); mbar_init(bar_p + 8 * w, 4); mbar_init(bar_p + 16 + 8 * w, 4); }
-        for (int w = 0; w < 2; w++) { mbar_init(bar_o + 8 * w, 1); mbar_init(bar_q + 8 * w, 4); mbar_init(bar_turn + 8 * w, 4); }
+        for (int w = 0; w < 2; w++) {
+            mbar_init(bar_s + 8 * w, 1); mbar_init(bar_s + 16 + 8 * w, 1);
+            mbar_init(bar_p + 8 * w, 4); mbar_init(bar_p + 16 + 8 * w, 4);
+            mbar_init(bar_v + 8 * w, 1); mbar_init(bar_o + 8 * w, 1); mbar_init(bar_q + 8 * w, 4);
+        }
         abort_flag_word = 0;
         odd_value = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -237,7 +249,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     PromptItem it;
-    const bool has_item = find_prompt_item<PR_THREADS>(a, (int)(blockIdx.x / p.splits), (int)(blockIdx.x % p.splits), p.splits, blockIdx.x == 0, &it, warp_sum, &item_shared);
+    const bool has_item = find_prompt_item<PR_THREADS>(a, (int)(blockIdx.x / p.splits), (int)(blockIdx.x % p.splits), p.splits, blockIdx.x == 0, &it, (FindSpace*)row_values);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -251,13 +263,6 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
     auto place_hi = [&](int w) { return first_place + over_group(p, it.row0 + min(128 * w + 127, it.rows - 1)); };
     auto block_token = [&](int j) { return key_block(it.kb, it.n0 + j) << 7; };
 
-    if (warp < PR_LOADER) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PR_REGS_SOFTMAX));
-    } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PR_REGS_OTHER));
-    }
-
-    // (each role ends by itself: behind the branches the roles' numbers of registers would differ)
     auto all_done = [] { asm volatile("bar.sync 1, %0;" ::"n"(PR_THREADS) : "memory"); };
     if (warp < PR_LOADER) {
         if (!work) { all_done(); return; }
@@ -288,185 +293,158 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
         __syncwarp();
         if (lane == 0) mbar_arrive(bar_q + 8 * w);
 
-        // ---- softmax: a row per thread ----
+        // ---- softmax: a row per thread, 64 tokens at a time ----
         const int i = 128 * w + tid;
         const bool mine = w < tiles && i < it.rows;
         const int packed = it.row0 + i, row = over_group(p, packed), place = first_place + row;
         const int lo = w < tiles ? place_lo(w) : 0, hi = w < tiles ? place_hi(w) : -1;
         const unsigned lanes = (unsigned)(warp & 3) << 21;              // lane quarter of tensor memory
-        const unsigned ts = tmem + w * 128 + lanes, to = tmem + 256 + w * D + lanes;
+        const unsigned to = tmem + 256 + w * D + lanes;
         const float c = a.scale_log2e;
         float m_used = -INFINITY, l = 0.0f;
-        unsigned phase = 0;
+        unsigned phase = 0, v_phase = 1;                                // v_phase: of the products with V that have been asked for
         bool alive = true, any = false;
-        // The two tiles take their exponentials in turns (tile 0, tile 1, tile 0, ...): side by side each would wait for the other's, and then both for their
-        // products.  One turn for each block, seen or not.
-        auto take_turn = [&](int j) {
-            if (tiles == 2 && (w == 1 || j > 0)) alive = alive && __all_sync(0xffffffffu, mbar_wait(bar_turn + 8 * w, (unsigned)(w == 1 ? j : j - 1) & 1, abort_flag, limit));
+        auto wait = [&](unsigned bar, unsigned parity) {
+            if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) alive = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit));
         };
-        auto pass_turn = [&] {
-            if (tiles == 2) {
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar_turn + 8 * (1 - w));
-            }
-        };
-        for (int j = 0; j < n && w < tiles; j++) {
+        for (int j = 0; j < n && w < tiles && alive; j++) {
             const int tok0 = block_token(j);
-            if (!(tok0 <= hi && (a.window == 0 || tok0 + 127 > lo - a.window || tok0 < a.sinks))) {
-                take_turn(j);
-                pass_turn();
-                continue;
-            }
-            alive = __all_sync(0xffffffffu, mbar_wait(bar_s + 8 * w, phase, abort_flag, limit));
-            if (!alive) break;
-            phase ^= 1;
-            tc_fence_after();
-            const volatile PromptMeta& mt = meta[j % PR_META];
-            const unsigned bad = mt.bad;
-            const bool whole = bad == 0 && tok0 + 127 <= lo && (a.window == 0 || tok0 > hi - a.window || tok0 + 127 < a.sinks);
-            // bit e of seen[q]: token tok0 + 32 q + e is seen
-            unsigned seen[4] = {0xffffffffu, 0xffffffffu, 0xffffffffu, 0xffffffffu};
-            if (!whole) {
-                const int to_hi = place - tok0, from = a.window ? place - a.window - tok0 : -1, sink = a.sinks > tok0 ? a.sinks - tok0 : 0;
-#pragma unroll
-                for (int q = 0; q < 4; q++) {
-                    seen[q] = first_bits(to_hi + 1 - 32 * q) & (~first_bits(from + 1 - 32 * q) | first_bits(sink - 32 * q));
-                    seen[q] &= ((bad >> (2 * q)) & 1 ? 0u : 0x0000ffffu) | ((bad >> (2 * q + 1)) & 1 ? 0u : 0xffff0000u);
-                }
-            }
-            // ---- the largest score, 32 columns at a time: the next ones are on their way meanwhile ----
-            unsigned xa[32], xb[32];
-            float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-            auto largest = [&](unsigned (&x)[32], int q) {
+            if (!(tok0 <= hi && (a.window == 0 || tok0 + 127 > lo - a.window || tok0 < a.sinks))) continue;
+#pragma unroll 1
+            for (int h = 0; h < 2; h++) {
+                wait(bar_s + 16 * h + 8 * w, phase);
+                if (!alive) break;
+                tc_fence_after();
+                const unsigned ts = tmem + w * 128 + 64 * h + lanes;
+                unsigned xa[32], xb[32];
+                tc_ld32(ts, xa);
+                tc_ld32(ts + 32, xb);
+                const volatile PromptMeta& mt = meta[j % PR_META];
+                const unsigned bad = mt.bad >> (4 * h) & 15u;
+                const int at = tok0 + 64 * h;
+                const bool whole = bad == 0 && at + 63 <= lo && (a.window == 0 || at > hi - a.window || at + 63 < a.sinks);
+                // bit e of seen[q]: token at + 32 q + e is seen
+                unsigned seen[2] = {0xffffffffu, 0xffffffffu};
                 if (!whole) {
+                    const int to_hi = place - at, from = a.window ? place - a.window - at : -1, sink = a.sinks > at ? a.sinks - at : 0;
 #pragma unroll
-                    for (int e = 0; e < 32; e++)
-                        if (!(seen[q] & (1u << e))) x[e] = 0xff800000u;
+                    for (int q = 0; q < 2; q++) {
+                        seen[q] = first_bits(to_hi + 1 - 32 * q) & (~first_bits(from + 1 - 32 * q) | first_bits(sink - 32 * q));
+                        seen[q] &= ((bad >> (2 * q)) & 1 ? 0u : 0x0000ffffu) | ((bad >> (2 * q + 1)) & 1 ? 0u : 0xffff0000u);
+                    }
                 }
-                if constexpr (S8) {
+                tc_wait_ld();
+                // ---- the largest score ----
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                auto largest = [&](unsigned (&x)[32], int q) {
+                    if (!whole) {
 #pragma unroll
-                    for (int g = 0; g < 2; g++) {                   // (factors are not negative; none seen stays -inf beside a factor of 0)
-                        float t0 = max3(__uint_as_float(x[16 * g]), __uint_as_float(x[16 * g + 1]), __uint_as_float(x[16 * g + 2]));
-                        float t1 = max3(__uint_as_float(x[16 * g + 3]), __uint_as_float(x[16 * g + 4]), __uint_as_float(x[16 * g + 5]));
+                        for (int e = 0; e < 32; e++)
+                            if (!(seen[q] & (1u << e))) x[e] = 0xff800000u;
+                    }
+                    if constexpr (S8) {
 #pragma unroll
-                        for (int e = 6; e < 16; e += 4) {
-                            t0 = max3(t0, __uint_as_float(x[16 * g + e]), __uint_as_float(x[16 * g + e + 1]));
-                            if (e + 2 < 16) t1 = max3(t1, __uint_as_float(x[16 * g + e + 2]), __uint_as_float(x[16 * g + e + 3]));
+                        for (int g = 0; g < 2; g++) {               // (factors are not negative; none seen stays -inf beside a factor of 0)
+                            float t0 = max3(__uint_as_float(x[16 * g]), __uint_as_float(x[16 * g + 1]), __uint_as_float(x[16 * g + 2]));
+                            float t1 = max3(__uint_as_float(x[16 * g + 3]), __uint_as_float(x[16 * g + 4]), __uint_as_float(x[16 * g + 5]));
+#pragma unroll
+                            for (int e = 6; e < 16; e += 4) {
+                                t0 = max3(t0, __uint_as_float(x[16 * g + e]), __uint_as_float(x[16 * g + e + 1]));
+                                if (e + 2 < 16) t1 = max3(t1, __uint_as_float(x[16 * g + e + 2]), __uint_as_float(x[16 * g + e + 3]));
+                            }
+                            t0 = max3(t0, t1, t1);
+                            top[2 * q + g] = t0 == -INFINITY ? t0 : t0 * mt.k[4 * h + 2 * q + g];
                         }
-                        t0 = max3(t0, t1, t1);
-                        top[g] = max3(top[g], t0 == -INFINITY ? t0 : t0 * mt.k[2 * q + g], top[g + 2]);
-                    }
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 32; e += 8)
-#pragma unroll
-                        for (int u = 0; u < 4; u++) top[u] = max3(top[u], __uint_as_float(x[e + 2 * u]), __uint_as_float(x[e + 2 * u + 1]));
-                }
-            };
-            tc_ld32(ts, xa);
-            tc_wait_ld();
-            tc_ld32(ts + 32, xb);
-            largest(xa, 0);
-            tc_wait_ld();
-            tc_ld32(ts + 64, xa);
-            largest(xb, 1);
-            tc_wait_ld();
-            tc_ld32(ts + 96, xb);
-            largest(xa, 2);
-            tc_wait_ld();
-            tc_ld32(ts, xa);
-            largest(xb, 3);
-            const float m_new = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * c;      // (c > 0)
-            const bool far = m_new > m_used + 8.0f;
-            if (__any_sync(0xffffffffu, far)) {
-                float f = 1.0f;
-                if (far) { f = exp2_approx(m_used - m_new); m_used = m_new; }
-                l *= f;
-                if (any) {
-                    // (the products into O up to the block before are complete: S of this block was issued behind them)
-#pragma unroll
-                    for (int q = 0; q < D / 16; q++) {
-                        unsigned y[16];
-                        tc_ld16(to + 16 * q, y);
-                        tc_wait_ld();
-#pragma unroll
-                        for (int e = 0; e < 16; e++) y[e] = __float_as_uint(__uint_as_float(y[e]) * f);
-                        tc_st16(to + 16 * q, y);
-                    }
-                }
-            }
-            any = true;
-            const float shift = m_used == -INFINITY ? 0.0f : -m_used;
-            const f32x2 c2 = pack2(c, c), s2 = pack2(shift, shift);
-            f32x2 sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
-            // ---- probabilities of 32 columns, over the columns of S that have been read ----
-            auto weigh = [&](const unsigned (&x)[32], int q, auto all) {
-                constexpr bool ALL = decltype(all)::value != 0;
-                unsigned pk[16];
-#pragma unroll
-                for (int e = 0; e < 32; e += 2) {
-                    f32x2 f2 = c2;
-                    if constexpr (S8) {
-                        const float f = mt.k[2 * q + (e >> 4)] * c;
-                        f2 = pack2(f, f);
-                    }
-                    const f32x2 y2 = fma2(pack2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), f2, s2);
-                    float y0, y1;
-                    if (ALL && (e >> 1) % 4 < PR_POLY) {
-                        unpack2(exp2_poly2(y2), y0, y1);
                     } else {
-                        unpack2(y2, y0, y1);
-                        y0 = exp2_approx(y0); y1 = exp2_approx(y1);
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8)
+#pragma unroll
+                            for (int u = 0; u < 4; u++) top[u] = max3(top[u], __uint_as_float(x[e + 2 * u]), __uint_as_float(x[e + 2 * u + 1]));
                     }
-                    if (!ALL) {
-                        if (!(seen[q] & (1u << e))) y0 = 0.0f;
-                        if (!(seen[q] & (2u << e))) y1 = 0.0f;
+                };
+                largest(xa, 0);
+                largest(xb, 1);
+                const float m_new = max3(max3(top[0], top[1], top[2]), top[3], top[3]) * c;      // (c > 0)
+                const bool far = m_new > m_used + 8.0f;
+                if (__any_sync(0xffffffffu, far)) {
+                    float f = 1.0f;
+                    if (far) { f = exp2_approx(m_used - m_new); m_used = m_new; }
+                    l *= f;
+                    if (any) {
+                        wait(bar_v + 8 * w, v_phase);              // every product into O that has been asked for
+                        if (!alive) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int q = 0; q < D / 16; q++) {
+                            unsigned y[16];
+                            tc_ld16(to + 16 * q, y);
+                            tc_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 16; e++) y[e] = __float_as_uint(__uint_as_float(y[e]) * f);
+                            tc_st16(to + 16 * q, y);
+                        }
                     }
-                    sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pack2(y0, y1));
-                    if constexpr (S8) {
-                        const float f = mt.v[2 * q + (e >> 4)];
-                        unpack2(mul2(pack2(y0, y1), pack2(f, f)), y0, y1);
-                        if (!ALL) {                                  // (a masked token has no part in its page's factor, which may be NaN)
+                }
+                any = true;
+                v_phase ^= 1;
+                const float shift = m_used == -INFINITY ? 0.0f : -m_used;
+                const f32x2 c2 = pack2(c, c), s2 = pack2(shift, shift);
+                f32x2 sum[2] = {pack2(0.0f, 0.0f), pack2(0.0f, 0.0f)};
+                // ---- probabilities of 32 columns, over columns of S that have been read ----
+                auto weigh = [&](const unsigned (&x)[32], int q, auto all) {
+                    constexpr bool ALL = decltype(all)::value != 0;
+                    unsigned pk[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) {
+                        f32x2 f2 = c2;
+                        if constexpr (S8) {
+                            const float f = mt.k[4 * h + 2 * q + (e >> 4)] * c;
+                            f2 = pack2(f, f);
+                        }
+                        const f32x2 y2 = fma2(pack2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), f2, s2);
+                        float y0, y1;
+                        if (ALL && (e >> 1) % 4 < PR_POLY) {
+                            unpack2(exp2_poly2(y2), y0, y1);
+                        } else {
+                            unpack2(y2, y0, y1);
+                            y0 = exp2_approx(y0); y1 = exp2_approx(y1);
+                        }
+                        if (!ALL) {
                             if (!(seen[q] & (1u << e))) y0 = 0.0f;
                             if (!(seen[q] & (2u << e))) y1 = 0.0f;
                         }
+                        sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pack2(y0, y1));
+                        if constexpr (S8) {
+                            const float f = mt.v[4 * h + 2 * q + (e >> 4)];
+                            unpack2(mul2(pack2(y0, y1), pack2(f, f)), y0, y1);
+                            if (!ALL) {                              // (a masked token has no part in its page's factor, which may be NaN)
+                                if (!(seen[q] & (1u << e))) y0 = 0.0f;
+                                if (!(seen[q] & (2u << e))) y1 = 0.0f;
+                            }
+                        }
+                        pk[e >> 1] = pack_bf16x2(y0, y1);
                     }
-                    pk[e >> 1] = pack_bf16x2(y0, y1);
+                    tc_st16(ts + 16 * q, pk);
+                };
+                if (whole) {
+                    weigh(xa, 0, IntConst<1>());
+                    weigh(xb, 1, IntConst<1>());
+                } else {
+                    weigh(xa, 0, IntConst<0>());
+                    weigh(xb, 1, IntConst<0>());
                 }
-                tc_st16(ts + 16 * q, pk);
-            };
-            auto hand_over = [&](int h) {
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar_p + 16 * h + 8 * w);
-            };
-            take_turn(j);
-            if (!alive) break;
-            auto all_four = [&](auto all) {
-                tc_wait_ld();
-                tc_ld32(ts + 32, xb);
-                weigh(xa, 0, all);
-                tc_wait_ld();
-                tc_ld32(ts + 64, xa);
-                weigh(xb, 1, all);
-                tc_wait_ld();
-                tc_ld32(ts + 96, xb);
-                weigh(xa, 2, all);
-                hand_over(0);               // (its product with V runs under the last columns' exponentials; waited for here its stores cost nothing)
-                tc_wait_ld();
-                weigh(xb, 3, all);
-                pass_turn();
-                hand_over(1);
-            };
-            if (whole) all_four(IntConst<1>());
-            else all_four(IntConst<0>());
-            float a0, a1, b0, b1;
-            unpack2(sum[0], a0, a1); unpack2(sum[1], b0, b1);
-            l += (a0 + a1) + (b0 + b1);
+                float a0, a1, b0, b1;
+                unpack2(sum[0], a0, a1); unpack2(sum[1], b0, b1);
+                l += (a0 + a1) + (b0 + b1);
+            }
+            phase ^= 1;
         }
         // ---- O ----
-        if (any && alive) alive = __all_sync(0xffffffffu, mbar_wait(bar_o + 8 * w, 0, abort_flag, limit));
+        if (any && alive) wait(bar_o + 8 * w, 0);
         tc_fence_after();
         if (alive && w < tiles && !*(volatile int*)&odd_value) {
             const float inv = split ? 1.0f : (l != 0.0f ? 1.0f / l : 0.0f);
@@ -677,7 +655,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
     } else if (warp < PR_MMA + 2) {
         // ---- products of tile w ----
         const int w = warp - PR_MMA;
-        const unsigned idesc_s = make_idesc_bf16(PR_BLOCK, false), idesc_o = make_idesc_bf16(D, true);
+        const unsigned idesc_s = make_idesc_bf16(PR_BLOCK / 2, false), idesc_o = make_idesc_bf16(D, true);
         const int lo = place_lo(w), hi = place_hi(w);
         auto needed = [&](int j) {
             const int tok0 = block_token(j);
@@ -687,7 +665,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
         bool alive = work && n > 0 && w < tiles, begun = false;
         unsigned p_phase = 0, phase = 0;                     // phase: of the ring, at slot `slot`
         int slot = 0;
-        const unsigned ts = tmem + w * 128, to = tmem + 256 + w * D, bs = bar_s + 8 * w, bp = bar_p + 8 * w;
+        const unsigned ts = tmem + w * 128, to = tmem + 256 + w * D, bs = bar_s + 8 * w, bp = bar_p + 8 * w, bv = bar_v + 8 * w;
         const unsigned long long q_desc = make_smem_desc(smem_u32(smem + w * SM::TILE)), k_desc = make_smem_desc(smem_u32(ring)),
                                  v_desc = make_smem_desc_nmajor(smem_u32(ring), HALF);
         auto wait = [&](unsigned bar, unsigned parity) { alive = alive && __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit)); };
@@ -700,56 +678,53 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
             }
         };
         auto step = [&](int& at, unsigned& ph) { if (++at == SLOTS) { at = 0; ph ^= 1; } };
-        auto scores = [&](unsigned long long kd) {           // by one lane
+        // by one lane: S of half h of a block's tokens; and the product of its probabilities with V
+        auto scores = [&](unsigned long long kd, int h) {
 #pragma unroll
             for (int k = 0; k < D / 16; k++) {
                 const unsigned long long off = (unsigned long long)((k >> 2) * (HALF >> 4) + (k & 3) * 2);
-                tc_mma<false>(ts, q_desc + off, kd + off, idesc_s, (unsigned)(k != 0));
+                tc_mma<false>(ts + 64 * h, q_desc + off, kd + off + (unsigned long long)(h * (64 * 128 >> 4)), idesc_s, (unsigned)(k != 0));
             }
-            tc_commit(bs);
+            tc_commit(bs + 16 * h);
         };
-        auto weighted = [&](unsigned long long vd, int h) {  // by one lane: half of the block's tokens
+        auto weighted = [&](unsigned long long vd, int h) {
 #pragma unroll
-            for (int k = 4 * h; k < 4 * h + 4; k++) tc_mma_ts(to, ts + k * 8, vd + (unsigned long long)(k * (2048 >> 4)), idesc_o, (unsigned)(begun || k != 0));
+            for (int k = 0; k < 4; k++)
+                tc_mma_ts(to, ts + 64 * h + k * 8, vd + (unsigned long long)((4 * h + k) * (2048 >> 4)), idesc_o, (unsigned)(begun || h != 0 || k != 0));
+            tc_commit(bv);
         };
         wait(bar_q + 8 * w, 0);
         wait(bar_full, 0);
         bool need = alive && needed(0);
         if (alive) {
             tc_fence_after();
-            if (need && elect_one()) scores(k_desc);
+            if (need && elect_one()) { scores(k_desc, 0); scores(k_desc, 1); }
             free_slot(0, need);
             step(slot, phase);
         }
         for (int j = 0; j < n && alive; j++) {
-            // fills 2 j + 1 (V of this block) and 2 j + 2 (K of the next).  Everything that can be known is known before the last probabilities come:
-            // between them and the next scores there is nothing but products
+            // fills 2 j + 1 (V of this block) and 2 j + 2 (K of the next).  Everything that can be known is known before the probabilities come: between them
+            // and the next scores in their place there is nothing but products
             const int vs = slot;
             wait(bar_full + 8 * slot, phase);
             step(slot, phase);
             const unsigned long long vd = v_desc + (unsigned long long)(vs * (SM::TILE >> 4)), kd = k_desc + (unsigned long long)(slot * (SM::TILE >> 4));
             const bool last = j + 1 == n, next = !last && needed(j + 1);
-            if (need) {
-                wait(bp, p_phase);
-                if (!alive) break;
-                tc_fence_after();
-                if (elect_one()) weighted(vd, 0);
-            }
             if (!last) wait(bar_full + 8 * slot, phase);
-            if (need) {
-                wait(bp + 16, p_phase);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                if (need) wait(bp + 16 * h, p_phase);
                 if (!alive) break;
                 tc_fence_after();
                 if (elect_one()) {
-                    weighted(vd, 1);
-                    if (next) scores(kd);
+                    if (need) weighted(vd, h);
+                    if (next) scores(kd, h);
                 }
+            }
+            if (!alive) break;
+            if (need) {
                 p_phase ^= 1;
                 begun = true;
-            } else {
-                if (!alive) break;
-                tc_fence_after();
-                if (next && elect_one()) scores(kd);
             }
             free_slot(vs, need);
             if (!last) {
@@ -776,12 +751,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
 constexpr int PRC_CTAS = 16;      // CTAs of a tile: 16 rows each
 template <int D>
 __global__ void __launch_bounds__(128) paged_prompt_combine_kernel(const PromptParams p) {
-    __shared__ int warp_sum[4];
-    __shared__ PromptItem item_shared;
+    __shared__ FindSpace space;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const PagedAttn& a = p.a;
     PromptItem it;
-    if (!find_prompt_item<128>(a, (int)(blockIdx.x / PRC_CTAS), 0, p.splits, false, &it, warp_sum, &item_shared) || it.splits < 2) return;
+    if (!find_prompt_item<128>(a, (int)(blockIdx.x / PRC_CTAS), 0, p.splits, false, &it, &space) || it.splits < 2) return;
     const int lane = threadIdx.x & 31;
     constexpr int N = D / 32;
     for (int i = blockIdx.x % PRC_CTAS * 4 + (threadIdx.x >> 5); i < it.rows; i += PRC_CTAS * 4) {
@@ -847,7 +821,7 @@ int launch_paged_prompt(PagedAttn a, float scale, cudaStream_t s) {
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     p.splits = (int)std::max(1LL, std::min<long long>(std::min<long long>(16, sms / items), (a.c.capacity / PR_BLOCK + 1) / 2));
-    if (items * p.splits > 0x7fffffffLL / PRC_CTAS) { set_error("paged_attention: too many rows and heads for one call"); return B200FC_ERR_INVALID; }
+    if (items * p.splits > 1 << 25) { set_error("paged_attention: too many rows and heads for one call"); return B200FC_ERR_INVALID; }
     CUtensorMap maps[2] = {};
     p.tma = !S8 && make_page_map(&maps[0], a.c.k, D, a.c) && make_page_map(&maps[1], a.c.v, D, a.c);
     void* ws = nullptr;
