@@ -20,11 +20,14 @@ namespace b200fc {
 
 namespace {
 
-constexpr int PR_THREADS = 448;
+constexpr int PR_THREADS = 512;                    // (the last two warps only fill their group of four)
 constexpr int PR_ROWS = 256, PR_BLOCK = 128;       // packed rows of a CTA, tokens of a block
-constexpr int PR_LOADER = 8, PR_MMA = 12;          // first warps of these roles (the last one does nothing else)
-constexpr int PR_POLY = 0;                         // of four pairs of exponentials, those by polynomial
+constexpr int PR_LOADER = 8, PR_MMA = 12;          // first warps of these roles
 constexpr int PR_META = 8;                         // blocks whose facts are kept; more than the ring holds
+
+constexpr int PR_REGS = 128, PR_REGS_SOFTMAX = 152, PR_REGS_OTHER = 104;      // a thread, at launch and in the roles
+static_assert(PR_REGS_SOFTMAX * PR_LOADER * 32 + PR_REGS_OTHER * (PR_THREADS - PR_LOADER * 32) <= PR_REGS * PR_THREADS && PR_REGS * PR_THREADS <= 65536,
+              "the split must not ask for more than the launch has");
 
 template <int D> struct PromptSmem {
     static constexpr int HALF = PR_BLOCK * 128;                       // 128 rows of 64 components
@@ -37,7 +40,9 @@ template <int D> struct PromptSmem {
     static constexpr int BYTES = ROWS + 2 * 128 * 2 * 4;              // (D = 128: all there is)
     static_assert(BYTES <= 232448, "shared memory of a CTA");
 };
-struct PromptMeta { unsigned bad; float k[8], v[8]; float pad[3]; };  // of a block: granules of 16 tokens that lie in no page of the pool; factors times 64
+// Of a block: its first token; granules of 16 tokens that lie in no page of the pool (bits 0-7), whether tile w sees any of it (bit 8 + w) and all rows of the
+// tile all of half h (bit 16 + 2 w + h); factors times 64.  Worked out once, by the warps that fetch it.
+struct PromptMeta { int tok0; unsigned facts; float k[8], v[8]; float pad[2]; };
 static_assert(sizeof(PromptMeta) == 80, "");
 
 struct PromptParams {
@@ -85,25 +90,6 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
 }
 // the lowest n bits, none or all of them beyond 0 .. 32
 __device__ __forceinline__ unsigned first_bits(int n) { return n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u); }
-// 2^x for two numbers up to 2^7 without the unit that computes ex2 (16 per clock and SM: it would need as long as the products): x = n + r with
-// |r| <= 1/2 by adding 1.5 * 2^23, 2^r by its minimax polynomial of degree 3 (Remez exchange; relative error 7.5e-5, a twenty-fifth of the rounding to
-// bf16 that follows), n + 100 added to the exponent, and a product with 2^-100 that lets what is below fp32's normal numbers become 0.
-__device__ __forceinline__ f32x2 exp2_poly2(f32x2 x) {
-    const f32x2 magic = pack2(12583012.0f, 12583012.0f), minus = pack2(-12583012.0f, -12583012.0f);      // 1.5 * 2^23 + 100
-    float x0, x1;
-    unpack2(x, x0, x1);
-    x = pack2(fmaxf(x0, -200.0f), fmaxf(x1, -200.0f));
-    const f32x2 t = add2(x, magic), r = fma2(add2(t, minus), pack2(-1.0f, -1.0f), x);
-    f32x2 q = fma2(r, pack2(0.055171669f, 0.055171669f), pack2(0.242611122f, 0.242611122f));
-    q = fma2(q, r, pack2(0.693260985f, 0.693260985f));
-    q = fma2(q, r, pack2(0.999928074f, 0.999928074f));
-    float t0, t1, q0, q1;
-    unpack2(t, t0, t1);
-    unpack2(q, q0, q1);
-    q = pack2(__uint_as_float(__float_as_uint(q0) + (__float_as_uint(t0) << 23)), __uint_as_float(__float_as_uint(q1) + (__float_as_uint(t1) << 23)));
-    asm("mul.rn.ftz.f32x2 %0, %0, %1;" : "+l"(q) : "l"(pack2(0x1p-100f, 0x1p-100f)));
-    return q;
-}
 __device__ __forceinline__ void fence_proxy_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // n / G for n < 2^31: the product with ceil(2^32 / G) is at most one too large
@@ -263,6 +249,12 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
     auto place_hi = [&](int w) { return first_place + over_group(p, it.row0 + min(128 * w + 127, it.rows - 1)); };
     auto block_token = [&](int j) { return key_block(it.kb, it.n0 + j) << 7; };
 
+    if (warp < PR_LOADER) {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PR_REGS_SOFTMAX));
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PR_REGS_OTHER));
+    }
+    // (each role ends by itself: behind the branches the roles' numbers of registers would differ)
     auto all_done = [] { asm volatile("bar.sync 1, %0;" ::"n"(PR_THREADS) : "memory"); };
     if (warp < PR_LOADER) {
         if (!work) { all_done(); return; }
@@ -297,7 +289,6 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
         const int i = 128 * w + tid;
         const bool mine = w < tiles && i < it.rows;
         const int packed = it.row0 + i, row = over_group(p, packed), place = first_place + row;
-        const int lo = w < tiles ? place_lo(w) : 0, hi = w < tiles ? place_hi(w) : -1;
         const unsigned lanes = (unsigned)(warp & 3) << 21;              // lane quarter of tensor memory
         const unsigned to = tmem + 256 + w * D + lanes;
         const float c = a.scale_log2e;
@@ -308,25 +299,27 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
             if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) alive = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit));
         };
         for (int j = 0; j < n && w < tiles && alive; j++) {
-            const int tok0 = block_token(j);
-            if (!(tok0 <= hi && (a.window == 0 || tok0 + 127 > lo - a.window || tok0 < a.sinks))) continue;
+            const volatile PromptMeta& mt = meta[j % PR_META];
 #pragma unroll 1
             for (int h = 0; h < 2; h++) {
+                const unsigned bp = bar_p + 16 * h + 8 * w, ts = tmem + w * 128 + 64 * h + lanes;
                 wait(bar_s + 16 * h + 8 * w, phase);
                 if (!alive) break;
                 tc_fence_after();
-                const unsigned ts = tmem + w * 128 + 64 * h + lanes;
+                const unsigned facts = mt.facts;
+                if (!(facts & 256u << w)) {
+                    if (lane == 0) mbar_arrive(bp);
+                    continue;
+                }
                 unsigned xa[32], xb[32];
                 tc_ld32(ts, xa);
                 tc_ld32(ts + 32, xb);
-                const volatile PromptMeta& mt = meta[j % PR_META];
-                const unsigned bad = mt.bad >> (4 * h) & 15u;
-                const int at = tok0 + 64 * h;
-                const bool whole = bad == 0 && at + 63 <= lo && (a.window == 0 || at > hi - a.window || at + 63 < a.sinks);
-                // bit e of seen[q]: token at + 32 q + e is seen
+                const bool whole = facts & 65536u << (2 * w + h);
+                // bit e of seen[q]: token tok0 + 64 h + 32 q + e is seen
                 unsigned seen[2] = {0xffffffffu, 0xffffffffu};
                 if (!whole) {
-                    const int to_hi = place - at, from = a.window ? place - a.window - at : -1, sink = a.sinks > at ? a.sinks - at : 0;
+                    const int at = mt.tok0 + 64 * h, to_hi = place - at, from = a.window ? place - a.window - at : -1, sink = a.sinks > at ? a.sinks - at : 0;
+                    const unsigned bad = facts >> (4 * h);
 #pragma unroll
                     for (int q = 0; q < 2; q++) {
                         seen[q] = first_bits(to_hi + 1 - 32 * q) & (~first_bits(from + 1 - 32 * q) | first_bits(sink - 32 * q));
@@ -393,7 +386,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
                 // ---- probabilities of 32 columns, over columns of S that have been read ----
                 auto weigh = [&](const unsigned (&x)[32], int q, auto all) {
                     constexpr bool ALL = decltype(all)::value != 0;
-                    unsigned pk[16];
+                    float y[32];
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
                         f32x2 f2 = c2;
@@ -401,29 +394,29 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
                             const float f = mt.k[4 * h + 2 * q + (e >> 4)] * c;
                             f2 = pack2(f, f);
                         }
-                        const f32x2 y2 = fma2(pack2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), f2, s2);
-                        float y0, y1;
-                        if (ALL && (e >> 1) % 4 < PR_POLY) {
-                            unpack2(exp2_poly2(y2), y0, y1);
-                        } else {
-                            unpack2(y2, y0, y1);
-                            y0 = exp2_approx(y0); y1 = exp2_approx(y1);
-                        }
-                        if (!ALL) {
-                            if (!(seen[q] & (1u << e))) y0 = 0.0f;
-                            if (!(seen[q] & (2u << e))) y1 = 0.0f;
-                        }
-                        sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pack2(y0, y1));
-                        if constexpr (S8) {
+                        unpack2(fma2(pack2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), f2, s2), y[e], y[e + 1]);
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; e++) {
+                        y[e] = exp2_approx(y[e]);
+                        if (!ALL && !(seen[q] & (1u << e))) y[e] = 0.0f;
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pack2(y[e], y[e + 1]));
+                    if constexpr (S8) {
+#pragma unroll
+                        for (int e = 0; e < 32; e += 2) {
                             const float f = mt.v[4 * h + 2 * q + (e >> 4)];
-                            unpack2(mul2(pack2(y0, y1), pack2(f, f)), y0, y1);
+                            unpack2(mul2(pack2(y[e], y[e + 1]), pack2(f, f)), y[e], y[e + 1]);
                             if (!ALL) {                              // (a masked token has no part in its page's factor, which may be NaN)
-                                if (!(seen[q] & (1u << e))) y0 = 0.0f;
-                                if (!(seen[q] & (2u << e))) y1 = 0.0f;
+                                if (!(seen[q] & (1u << e))) y[e] = 0.0f;
+                                if (!(seen[q] & (2u << e))) y[e + 1] = 0.0f;
                             }
                         }
-                        pk[e >> 1] = pack_bf16x2(y0, y1);
                     }
+                    unsigned pk[16];
+#pragma unroll
+                    for (int e = 0; e < 32; e += 2) pk[e >> 1] = pack_bf16x2(y[e], y[e + 1]);
                     tc_st16(ts + 16 * q, pk);
                 };
                 if (whole) {
@@ -436,7 +429,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
                 tc_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(bar_p + 16 * h + 8 * w);
+                if (lane == 0) mbar_arrive(bp);
                 float a0, a1, b0, b1;
                 unpack2(sum[0], a0, a1); unpack2(sum[1], b0, b1);
                 l += (a0 + a1) + (b0 + b1);
@@ -505,6 +498,21 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
         const int r0 = tid / CH, ch = tid % CH, psh = a.c.page_shift;
         const int lo = place_lo(0), hi = place_hi(tiles - 1);
         int next_page = -1;
+        const int lo_of[2] = {lo, place_lo(1)}, hi_of[2] = {place_hi(0), hi};
+        auto facts = [&](int tok0, unsigned bad) {
+            unsigned f = bad;
+#pragma unroll
+            for (int w = 0; w < 2; w++) {
+                if (w >= tiles) continue;
+                if (tok0 <= hi_of[w] && (a.window == 0 || tok0 + 127 > lo_of[w] - a.window || tok0 < a.sinks)) f |= 256u << w;
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int at = tok0 + 64 * h;
+                    if ((bad >> (4 * h) & 15u) == 0 && at + 63 <= lo_of[w] && (a.window == 0 || at > hi_of[w] - a.window || at + 63 < a.sinks)) f |= 65536u << (2 * w + h);
+                }
+            }
+            return f;
+        };
         auto look_up = [&](int j) {                        // lane g < 8: page of granule g of block j
             next_page = -1;
             if (j < n && lane < 8) {
@@ -542,7 +550,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
             for (int j = 0; j < n && alive; j++) {
                 const int tok0 = block_token(j), page = next_page;
                 const unsigned bad = __ballot_sync(0xffffffffu, lane < 8 && page < 0) & 255u;
-                if (tid == 0) meta[j % PR_META].bad = bad;
+                if (tid == 0) {
+                    meta[j % PR_META].tok0 = tok0;
+                    meta[j % PR_META].facts = facts(tok0, bad);
+                }
                 look_up(j + 1);
                 // blocks that all rows see come by TMA, the others token by token with zeros for those that nobody sees
                 const bool plain = p.tma && bad == 0 && tok0 + 127 <= lo && (a.window == 0 || tok0 > hi - a.window || tok0 + 127 < a.sinks);
@@ -617,7 +628,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
                         meta[j % PR_META].k[lane] = page < 0 ? 0.0f : 64.0f * __ldg(a.c.k_scale + at);
                         meta[j % PR_META].v[lane] = page < 0 ? 0.0f : 64.0f * __ldg(a.c.v_scale + at);
                     }
-                    if (lane == 0) meta[j % PR_META].bad = bad;
+                    if (lane == 0) {
+                        meta[j % PR_META].tok0 = block_token(j);
+                        meta[j % PR_META].facts = facts(block_token(j), bad);
+                    }
                 }
                 const int tok0 = block_token(j);
                 look_up(j + 1);
@@ -656,11 +670,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
         // ---- products of tile w ----
         const int w = warp - PR_MMA;
         const unsigned idesc_s = make_idesc_bf16(PR_BLOCK / 2, false), idesc_o = make_idesc_bf16(D, true);
-        const int lo = place_lo(w), hi = place_hi(w);
-        auto needed = [&](int j) {
-            const int tok0 = block_token(j);
-            return tok0 <= hi && (a.window == 0 || tok0 + 127 > lo - a.window || tok0 < a.sinks);
-        };
+        auto needed = [&](int j) { return (meta[j % PR_META].facts & 256u << w) != 0; };       // (of a block whose K has arrived)
         const int frees = tiles == 1 ? 2 : 1;                // arrivals of this tile on a slot's barrier (a lone tile's for both)
         bool alive = work && n > 0 && w < tiles, begun = false;
         unsigned p_phase = 0, phase = 0;                     // phase: of the ring, at slot `slot`
@@ -679,7 +689,12 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
         };
         auto step = [&](int& at, unsigned& ph) { if (++at == SLOTS) { at = 0; ph ^= 1; } };
         // by one lane: S of half h of a block's tokens; and the product of its probabilities with V
-        auto scores = [&](unsigned long long kd, int h) {
+        // (every half of every block is handed back and forth, seen or not: so no side can be two steps ahead on a barrier)
+        auto scores = [&](unsigned long long kd, int h, bool some) {
+            if (!some) {
+                mbar_arrive(bs + 16 * h);
+                return;
+            }
 #pragma unroll
             for (int k = 0; k < D / 16; k++) {
                 const unsigned long long off = (unsigned long long)((k >> 2) * (HALF >> 4) + (k & 3) * 2);
@@ -698,7 +713,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
         bool need = alive && needed(0);
         if (alive) {
             tc_fence_after();
-            if (need && elect_one()) { scores(k_desc, 0); scores(k_desc, 1); }
+            if (elect_one()) {
+                scores(k_desc, 0, need);
+                scores(k_desc, 1, need);
+            }
             free_slot(0, need);
             step(slot, phase);
         }
@@ -709,23 +727,22 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
             wait(bar_full + 8 * slot, phase);
             step(slot, phase);
             const unsigned long long vd = v_desc + (unsigned long long)(vs * (SM::TILE >> 4)), kd = k_desc + (unsigned long long)(slot * (SM::TILE >> 4));
-            const bool last = j + 1 == n, next = !last && needed(j + 1);
+            const bool last = j + 1 == n;
             if (!last) wait(bar_full + 8 * slot, phase);
+            const bool next = !last && alive && needed(j + 1);
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                if (need) wait(bp + 16 * h, p_phase);
+                wait(bp + 16 * h, p_phase);
                 if (!alive) break;
                 tc_fence_after();
                 if (elect_one()) {
                     if (need) weighted(vd, h);
-                    if (next) scores(kd, h);
+                    if (!last) scores(kd, h, next);
                 }
             }
             if (!alive) break;
-            if (need) {
-                p_phase ^= 1;
-                begun = true;
-            }
+            p_phase ^= 1;
+            begun = begun || need;
             free_slot(vs, need);
             if (!last) {
                 free_slot(slot, next);
