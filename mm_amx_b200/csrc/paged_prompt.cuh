@@ -6,9 +6,9 @@
 //   warps 0-3, 4-7   softmax of tile 0, 1: a thread has one row.  S comes from tensor memory 64 tokens at a time, exp2(S - max) goes back over it as bf16.  The
 //                    maximum that is subtracted follows the true one only when that is 2^8 ahead (sums and values are fp32 and stay far from their limits, the
 //                    probabilities' rounding is relative), so that O in tensor memory is rescaled hardly ever.
-//   warps 8-11       fetch K and V blocks into a ring of 128-token slots (128-byte swizzle): bf16 by TMA, or in blocks that not every row sees by cp.async with zeros
+//   4 or 8 more      fetch K and V blocks into a ring of 128-token slots (128-byte swizzle): bf16 by TMA, or in blocks that not every row sees by cp.async with zeros
 //                    for tokens that nobody sees (which may hold anything), 8 bits widened on the way to bf16 of (value / 64), exactly; the page's factors go to the softmax.
-//   warps 12, 13     issue the products of tile 0, 1: S_w = Q_w K^T (Q, K in shared memory), O_w += P_w V (P in tensor memory, V as it lies: N-major).  One
+//   two more         issue the products of tile 0, 1: S_w = Q_w K^T (Q, K in shared memory), O_w += P_w V (P in tensor memory, V as it lies: N-major).  One
 //                    tile's products run under the other tile's softmax.  (One warp for both tiles was the bottleneck: 3900 clocks a block.)
 // Tensor memory: S_0 S_1 (128 columns each; P over the first half of either 64) O_0 O_1 (D columns each).
 // A value that is no number in a block that some rows do not see would reach them as 0 * NaN: the fetching warps look for one in such blocks, and a CTA that
@@ -20,14 +20,18 @@ namespace b200fc {
 
 namespace {
 
-constexpr int PR_THREADS = 512;                    // (the last two warps only fill their group of four)
 constexpr int PR_ROWS = 256, PR_BLOCK = 128;       // packed rows of a CTA, tokens of a block
-constexpr int PR_LOADER = 8, PR_MMA = 12;          // first warps of these roles
+constexpr int PR_LOADER = 8;                       // first of the warps that fetch
 constexpr int PR_META = 8;                         // blocks whose facts are kept; more than the ring holds
 
-constexpr int PR_REGS = 128, PR_REGS_SOFTMAX = 152, PR_REGS_OTHER = 104;      // a thread, at launch and in the roles
-static_assert(PR_REGS_SOFTMAX * PR_LOADER * 32 + PR_REGS_OTHER * (PR_THREADS - PR_LOADER * 32) <= PR_REGS * PR_THREADS && PR_REGS * PR_THREADS <= 65536,
-              "the split must not ask for more than the launch has");
+// Warps and registers.  8 bits are widened by eight warps (with four they were the bottleneck: 185 us where this takes 155), bf16 needs four.  The last two warps
+// only fill their group of four.
+template <bool S8> struct PromptShape {
+    static constexpr int MMA = PR_LOADER + (S8 ? 8 : 4), THREADS = (MMA + 4) * 32;
+    static constexpr int REGS = S8 ? 96 : 128, REGS_SOFTMAX = 152, REGS_OTHER = S8 ? 56 : 104;      // a thread, at launch and in the roles
+    static_assert(REGS_SOFTMAX * PR_LOADER * 32 + REGS_OTHER * (THREADS - PR_LOADER * 32) <= REGS * THREADS && REGS * THREADS <= 65536,
+                  "the split must not ask for more than the launch has");
+};
 
 template <int D> struct PromptSmem {
     static constexpr int HALF = PR_BLOCK * 128;                       // 128 rows of 64 components
@@ -113,7 +117,7 @@ __device__ __forceinline__ int prompt_splits(int count, int splits) { return max
 constexpr int PR_RANKED = 64;
 struct FindSpace {
     PromptItem item;
-    int warp_sum[PR_THREADS / 32], keys[PR_RANKED], order[PR_RANKED];
+    int warp_sum[PromptShape<true>::THREADS / 32], keys[PR_RANKED], order[PR_RANKED];
 };
 static_assert(sizeof(FindSpace) <= 2048, "lies where the rows' values come later");
 template <int THREADS>
@@ -196,9 +200,10 @@ __device__ __forceinline__ bool find_prompt_item(const PagedAttn& a, int item, i
 }
 
 template <int D, bool S8>
-__global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PromptParams p) {
+__global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PromptParams p) {
     using SM = PromptSmem<D>;
-    constexpr int SLOTS = SM::SLOTS, HALF = SM::HALF;
+    using SH = PromptShape<S8>;
+    constexpr int SLOTS = SM::SLOTS, HALF = SM::HALF, PR_MMA = SH::MMA, PR_THREADS = SH::THREADS;
     // no static shared memory: the dynamic part then begins at a multiple of 1024, as the swizzle wants it
     extern __shared__ __align__(1024) unsigned char smem[];
     int& odd_value = *(int*)(smem + SM::BARS + 368);
@@ -219,7 +224,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
     const unsigned long long limit = p.wait_limit_ns;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < SLOTS; i++) { mbar_init(bar_full + 8 * i, 4); mbar_init(bar_empty + 8 * i, 2); }
+        for (int i = 0; i < SLOTS; i++) { mbar_init(bar_full + 8 * i, PR_MMA - PR_LOADER); mbar_init(bar_empty + 8 * i, 2); }
         for (int w = 0; w < 2; w++) {
             mbar_init(bar_s + 8 * w, 1); mbar_init(bar_s + 16 + 8 * w, 1);
             mbar_init(bar_p + 8 * w, 4); mbar_init(bar_p + 16 + 8 * w, 4);
@@ -250,9 +255,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
     auto block_token = [&](int j) { return key_block(it.kb, it.n0 + j) << 7; };
 
     if (warp < PR_LOADER) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PR_REGS_SOFTMAX));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(SH::REGS_SOFTMAX));
     } else {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PR_REGS_OTHER));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(SH::REGS_OTHER));
     }
     // (each role ends by itself: behind the branches the roles' numbers of registers would differ)
     auto all_done = [] { asm volatile("bar.sync 1, %0;" ::"n"(PR_THREADS) : "memory"); };
@@ -397,9 +402,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
                         unpack2(fma2(pack2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), f2, s2), y[e], y[e + 1]);
                     }
 #pragma unroll
-                    for (int e = 0; e < 32; e++) {
+                    for (int e = 0; e < 32; e += 2) {
                         y[e] = exp2_approx(y[e]);
+                        y[e + 1] = exp2_approx(y[e + 1]);
                         if (!ALL && !(seen[q] & (1u << e))) y[e] = 0.0f;
+                        if (!ALL && !(seen[q] & (2u << e))) y[e + 1] = 0.0f;
                     }
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pack2(y[e], y[e + 1]));
@@ -494,7 +501,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
         if (!work) { all_done(); return; }
         // ---- K and V: fill f = 2 j + (0 for K, 1 for V) goes to slot f % SLOTS ----
         const int tid = threadIdx.x - PR_LOADER * 32;
-        constexpr int CH = S8 ? D / 16 : D / 8, AT_ONCE = 128 / CH, STEPS = 128 / AT_ONCE;    // 16-byte chunks of a token; tokens that the warps take at once
+        constexpr int CH = S8 ? D / 16 : D / 8, AT_ONCE = (PR_MMA - PR_LOADER) * 32 / CH, STEPS = 128 / AT_ONCE;    // 16-byte chunks of a token; tokens that the warps take at once
         const int r0 = tid / CH, ch = tid % CH, psh = a.c.page_shift;
         const int lo = place_lo(0), hi = place_hi(tiles - 1);
         int next_page = -1;
@@ -544,8 +551,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar_full + 8 * (f % SLOTS));
             };
-            int pending = 0;                               // fills f - pending .. f - 1 are on their way by cp.async
             const long long ts = a.c.token_stride, thread_off = r0 * ts + ch * 16;
+            int pending = 0;                               // fills f - pending .. f - 1 are on their way by cp.async
             const unsigned thread_dst = smem_u32(ring) + (ch >> 3) * HALF + r0 * 128 + (((ch & 7) ^ (r0 & 7)) << 4);
             for (int j = 0; j < n && alive; j++) {
                 const int tok0 = block_token(j), page = next_page;
@@ -653,8 +660,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) paged_prompt_kernel(const __gri
                             o[2 * e + 1] = u8x2_to_bf16x2_64th(u, 0x4342);
                         }
                         unsigned char* d = dst + (ch >> 2) * HALF + r * 128;
-                        *(uint4*)(d + ((((2 * ch) & 7) ^ (r & 7)) << 4)) = make_uint4(o[0], o[1], o[2], o[3]);
-                        *(uint4*)(d + ((((2 * ch + 1) & 7) ^ (r & 7)) << 4)) = make_uint4(o[4], o[5], o[6], o[7]);
+                        // (threads of the second 64 components store their second chunk first: the two halves' banks are the same)
+                        const int first = ch >> 2 & 1;
+                        *(uint4*)(d + ((((2 * ch + first) & 7) ^ (r & 7)) << 4)) = first ? make_uint4(o[4], o[5], o[6], o[7]) : make_uint4(o[0], o[1], o[2], o[3]);
+                        *(uint4*)(d + ((((2 * ch + 1 - first) & 7) ^ (r & 7)) << 4)) = first ? make_uint4(o[0], o[1], o[2], o[3]) : make_uint4(o[4], o[5], o[6], o[7]);
                     }
                     // the next fill's bytes travel while this one is used
                     if (kv == 0) fetch(tok0, page, 1);
@@ -856,7 +865,7 @@ int launch_paged_prompt(PagedAttn a, float scale, cudaStream_t s) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(items * p.splits));
-    cfg.blockDim = dim3(PR_THREADS);
+    cfg.blockDim = dim3(PromptShape<S8>::THREADS);
     cfg.dynamicSmemBytes = SM::BYTES;
     cfg.stream = s;
     cfg.attrs = attr;
