@@ -288,7 +288,8 @@ int b200fc_decode_attention(const b200fc_attention_t* a, void* stream);
 /* A pool of pages of page_tokens tokens each, for Hkv kv heads of size D, and which of them the sequences of a call own.  Token t of sequence b
  * lies in page page_table[b][t / page_tokens] at place t % page_tokens:
  *     k + page * page_stride + head * head_stride + place * token_stride   (bytes; v has the same strides)
- * dtype B200FC_BF16, or B200FC_S8 with one fp32 factor for each page and kv head, in k_scale and v_scale: cached value = int8 * factor.
+ * dtype B200FC_BF16, or B200FC_S8 with one fp32 factor for each page and kv head, in k_scale and v_scale, not negative: cached value =
+ * int8 * factor.
  * D: 64 or 128.  page_tokens: 16, 32, 64 or 128.  k, v and their strides 16-byte aligned, token_stride >= a token's D elements.
  * Everything that page_table, seq_lens and row_start name is checked where it is read, on the device.  A sequence whose rows or length lie outside
  * their buffers is left out (its rows of out are not written), a page outside [0, pages) is neither written nor read, and the next

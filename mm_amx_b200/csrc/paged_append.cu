@@ -107,6 +107,26 @@ template <int D, bool S8>
 __device__ __forceinline__ void append_row(const AppendParams& p, int r, int group, int groups) {
     constexpr int ITEMS = D / 16, SLOTS = APP_THREADS / ITEMS;
     const int i = threadIdx.x % ITEMS, slot = threadIdx.x / ITEMS;
+    const Item it = item_of(p, i);
+    const int heads = p.H + (S8 ? 0 : 2 * p.c.Hkv), stride = groups * SLOTS;
+    auto source = [&](int h) {
+        if (h < p.H) return p.q + (long long)r * p.q_rs + (long long)h * p.q_hs;
+        const int hk = h - p.H;
+        return hk < p.c.Hkv ? p.k + (long long)r * p.k_rs + (long long)hk * p.k_hs : p.v + (long long)r * p.v_rs + (long long)(hk - p.c.Hkv) * p.v_hs;
+    };
+    // two heads at a time; the first two travel while the row's sequence, page and angles are looked up (5120 rows of 32 + 16 heads: 26 us without)
+    uint4 x[2][2];
+    auto load = [&](int h) {
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+            if (h + u * stride < heads) {
+                const unsigned char* src = source(h + u * stride);
+                x[u][0] = *(const uint4*)(src + 2 * it.lo);
+                x[u][1] = *(const uint4*)(src + 2 * it.hi);
+            }
+    };
+    int h = group * SLOTS + slot;
+    load(h);
     const int b = find_sequence(p.c, r);
     if (b < 0) return;
     SeqRows s;
@@ -117,34 +137,32 @@ __device__ __forceinline__ void append_row(const AppendParams& p, int r, int gro
     if (r < s.row0 || r >= s.row0 + s.rows) return;
     const int place = s.len - s.rows + (r - s.row0);
     if (place < 0) return;
-    const int heads = p.H + (S8 ? 0 : 2 * p.c.Hkv);
     const int page = S8 ? 0 : table_page(p.c, b, place >> p.c.page_shift);
-    const Item it = item_of(p, i);
     float cs[8], sn[8];
     bool ok = page >= 0;
     if (it.turned) ok = load_turn(p, i, r, place, cs, sn) && ok;
     if (!ok) report_paged(p.c);
     const long long token = (long long)(place & ((1 << p.c.page_shift) - 1)) * p.c.token_stride + (long long)page * p.c.page_stride;
-    for (int h = group * SLOTS + slot; h < heads; h += groups * SLOTS) {
-        const unsigned char* src;
-        unsigned char* dst;
-        bool turned = it.turned;
-        if (h < p.H) {
-            src = p.q + (long long)r * p.q_rs + (long long)h * p.q_hs;
-            dst = p.q_out + (long long)r * p.qo_rs + (long long)h * p.qo_hs;
-        } else {
-            if (page < 0) break;
-            const int hk = h - p.H;
-            const bool is_v = hk >= p.c.Hkv;
-            const int hh = is_v ? hk - p.c.Hkv : hk;
-            src = is_v ? p.v + (long long)r * p.v_rs + (long long)hh * p.v_hs : p.k + (long long)r * p.k_rs + (long long)hh * p.k_hs;
-            dst = (is_v ? p.c.v : p.c.k) + token + (long long)hh * p.c.head_stride;
-            turned = turned && !is_v;
+    for (; h < heads; h += 2 * stride, load(h))
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int hh = h + u * stride;
+            if (hh >= heads) break;
+            unsigned char* dst;
+            bool turned = it.turned;
+            if (hh < p.H) {
+                dst = p.q_out + (long long)r * p.qo_rs + (long long)hh * p.qo_hs;
+            } else {
+                if (page < 0) break;
+                const int hk = hh - p.H;
+                const bool is_v = hk >= p.c.Hkv;
+                dst = (is_v ? p.c.v : p.c.k) + token + (long long)(is_v ? hk - p.c.Hkv : hk) * p.c.head_stride;
+                turned = turned && !is_v;
+            }
+            float y[16];
+            turn(x[u][0], x[u][1], turned, p.interleaved, cs, sn, y);
+            store_bf16(dst, it, y);
         }
-        float y[16];
-        turn(*(const uint4*)(src + 2 * it.lo), *(const uint4*)(src + 2 * it.hi), turned, p.interleaved, cs, sn, y);
-        store_bf16(dst, it, y);
-    }
 }
 
 // four values -> int8, by the factor's reciprocal
@@ -154,6 +172,7 @@ __device__ __forceinline__ unsigned quant4(float a, float b, float c, float d, f
     return x | y << 8 | z << 16 | w << 24;
 }
 
+template <int N> struct Rounds { static constexpr int value = N; };
 // All new tokens of one page for a kv head, of k or of v.  segment: the how-manieth page that the call touches, over the sequences in order.
 template <int D>
 __device__ __forceinline__ void append_page(const AppendParams& p, int segment, int h, bool is_v) {
@@ -199,38 +218,81 @@ __device__ __forceinline__ void append_page(const AppendParams& p, int segment, 
     const int i = threadIdx.x % ITEMS, slot = threadIdx.x / ITEMS;
     Item it = item_of(p, i);
     it.turned = it.turned && !is_v;
-    auto values = [&](int t, float (&y)[16]) {
-        const int r = s.row0 + (t - (s.len - s.rows));
-        const unsigned char* x = src + (long long)r * rs;
-        float cs[8], sn[8];
-        if (it.turned && !load_turn(p, i, r, t, cs, sn)) report_paged(p.c);
-        turn(*(const uint4*)(x + 2 * it.lo), *(const uint4*)(x + 2 * it.hi), it.turned, p.interleaved, cs, sn, y);
+    // the rotated values of R of the thread's tokens, t0 and every SLOTS-th from there on; behind the last one the last one again, so that all loads travel
+    // together
+    auto values = [&](auto rounds, int t0, auto& y) {
+        constexpr int R = decltype(rounds)::value;
+        uint4 x[R][2];
+#pragma unroll
+        for (int n = 0; n < R; n++) {
+            const int t = min(t0 + n * SLOTS, hi - 1);
+            const unsigned char* row = src + (long long)(s.row0 + (t - (s.len - s.rows))) * rs;
+            x[n][0] = *(const uint4*)(row + 2 * it.lo);
+            x[n][1] = *(const uint4*)(row + 2 * it.hi);
+        }
+#pragma unroll
+        for (int n = 0; n < R; n++) {
+            const int t = min(t0 + n * SLOTS, hi - 1);
+            float cs[8], sn[8];
+            if (it.turned && !load_turn(p, i, s.row0 + (t - (s.len - s.rows)), t, cs, sn)) report_paged(p.c);
+            turn(x[n][0], x[n][1], it.turned, p.interleaved, cs, sn, y[n]);
+        }
     };
-    // ---- the largest new value, as bits: infinities and NaN are larger than any number ----
-    unsigned most = 0;
-    for (int t = lo + slot; t < hi; t += SLOTS) {
-        float y[16];
-        values(t, y);
+    unsigned most = 0;                                               // as bits: infinities and NaN are larger than any number
+    float after = 0.0f, inv = 0.0f;
+    auto largest = [&](auto rounds, const auto& y) {
 #pragma unroll
-        for (int j = 0; j < 16; j++) most = max(most, __float_as_uint(y[j]) & 0x7fffffffu);
-    }
-    most = __reduce_max_sync(0xffffffffu, most);
-    if (lane == 0) warp_max[threadIdx.x >> 5] = most;
-    __syncthreads();
+        for (int n = 0; n < decltype(rounds)::value; n++)
 #pragma unroll
-    for (int w = 0; w < APP_THREADS / 32; w++) most = max(most, warp_max[w]);
-    float after = fmaxf(before, __fdiv_rn(__uint_as_float(most), 127.0f));
-    if (after < FLT_MIN) after = 0.0f;                               // (its reciprocal would not be a number of fp32)
-    if (most >= 0x7f800000u || before != before) after = __uint_as_float(0x7fc00000u);
-    const float inv = after >= FLT_MIN ? __fdiv_rn(1.0f, after) : 0.0f;
-    if (threadIdx.x == 0) *factor = after;
-    // ---- store ----
-    for (int t = lo + slot; t < hi; t += SLOTS) {
-        float y[16];
-        values(t, y);
-        unsigned char* d = dst + (long long)(t - begin) * p.c.token_stride;
-        *(uint2*)(d + it.lo) = make_uint2(quant4(y[0], y[1], y[2], y[3], inv), quant4(y[4], y[5], y[6], y[7], inv));
-        *(uint2*)(d + it.hi) = make_uint2(quant4(y[8], y[9], y[10], y[11], inv), quant4(y[12], y[13], y[14], y[15], inv));
+            for (int j = 0; j < 16; j++) most = max(most, __float_as_uint(y[n][j]) & 0x7fffffffu);
+    };
+    auto settle = [&] {                                              // the page's factor, once the whole CTA knows its largest value
+        most = __reduce_max_sync(0xffffffffu, most);
+        if (lane == 0) warp_max[threadIdx.x >> 5] = most;
+        __syncthreads();
+#pragma unroll
+        for (int w = 0; w < APP_THREADS / 32; w++) most = max(most, warp_max[w]);
+        after = fmaxf(before, __fdiv_rn(__uint_as_float(most), 127.0f));
+        if (after < FLT_MIN) after = 0.0f;                           // (its reciprocal would not be a number of fp32)
+        if (most >= 0x7f800000u || before != before) after = __uint_as_float(0x7fc00000u);
+        inv = after >= FLT_MIN ? __fdiv_rn(1.0f, after) : 0.0f;
+        if (threadIdx.x == 0) *factor = after;
+    };
+    auto store = [&](auto rounds, int t0, const auto& y) {
+#pragma unroll
+        for (int n = 0; n < decltype(rounds)::value; n++) {
+            const int t = t0 + n * SLOTS;
+            if (t >= hi) break;
+            unsigned char* d = dst + (long long)(t - begin) * p.c.token_stride;
+            *(uint2*)(d + it.lo) = make_uint2(quant4(y[n][0], y[n][1], y[n][2], y[n][3], inv), quant4(y[n][4], y[n][5], y[n][6], y[n][7], inv));
+            *(uint2*)(d + it.hi) = make_uint2(quant4(y[n][8], y[n][9], y[n][10], y[n][11], inv), quant4(y[n][12], y[n][13], y[n][14], y[n][15], inv));
+        }
+    };
+    constexpr int R = 4;
+    if (hi - lo <= SLOTS) {                                          // a few tokens: one each
+        float y[1][16];
+        values(Rounds<1>(), lo + slot, y);
+        largest(Rounds<1>(), y);
+        settle();
+        store(Rounds<1>(), lo + slot, y);
+    } else if (hi - lo <= R * SLOTS) {                               // the values stay in registers
+        float y[R][16];
+        values(Rounds<R>(), lo + slot, y);
+        largest(Rounds<R>(), y);
+        settle();
+        store(Rounds<R>(), lo + slot, y);
+    } else {                                                         // (pages of 128 tokens of 128 components: everything twice)
+        for (int t0 = lo + slot; t0 - slot < hi; t0 += R * SLOTS) {
+            float y[R][16];
+            values(Rounds<R>(), t0, y);
+            largest(Rounds<R>(), y);
+        }
+        settle();
+        for (int t0 = lo + slot; t0 - slot < hi; t0 += R * SLOTS) {
+            float y[R][16];
+            values(Rounds<R>(), t0, y);
+            store(Rounds<R>(), t0, y);
+        }
     }
     if (!(after > before) || !has_old) return;
     for (int t = slot; t < lo - begin; t += SLOTS) {

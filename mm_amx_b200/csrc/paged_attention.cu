@@ -26,7 +26,8 @@ int launch_paged_attention(const b200fc_paged_attention_t& a, cudaStream_t s) {
     p.q = (const unsigned char*)a.q; p.q_rs = a.q_row_stride; p.q_hs = a.q_head_stride;
     p.out = (unsigned char*)a.out; p.o_rs = a.out_row_stride; p.o_hs = a.out_head_stride;
     p.H = a.H; p.G = a.H / c.Hkv;
-    p.window = a.window; p.sinks = a.sinks;
+    p.window = a.window < p.c.capacity ? a.window : 0;        // (a window as long as the cache is none)
+    p.sinks = a.sinks;
     p.scale_log2e = a.scale * 1.4426950408889634f;
     const bool s8 = c.dtype == B200FC_S8;
     p.c.max_rows = a.row_start ? std::min(a.max_rows, a.T) : 1;

@@ -250,7 +250,7 @@ __global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kern
     const bool work = has_item && (n > 0 || (it.kb.count == 0 && blockIdx.x % p.splits == 0));
     // places of a tile's first and last row, and which blocks it sees any of
     const int first_place = has_item ? it.s.len - it.s.rows : 0;
-    auto place_lo = [&](int w) { return first_place + over_group(p, it.row0 + 128 * w); };
+    auto place_lo = [&](int w) { return max(first_place + over_group(p, it.row0 + 128 * w), 0); };      // (rows in front of the first token see nothing)
     auto place_hi = [&](int w) { return first_place + over_group(p, it.row0 + min(128 * w + 127, it.rows - 1)); };
     auto block_token = [&](int j) { return key_block(it.kb, it.n0 + j) << 7; };
 

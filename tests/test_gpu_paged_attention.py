@@ -54,10 +54,25 @@ PROMPTS = [([100], [100], 2, 2, 64, 16), ([128, 256, 129], [128, 256, 129], 1, 4
 
 @pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
 @pytest.mark.parametrize("rows,lens,Hkv,G,D,page", PROMPTS, ids=str)
-@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (130, 5), (500, 300)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (1, 0), (130, 5), (500, 300), (2 ** 31 - 1, 2)])
 def test_prompts(rows, lens, Hkv, G, D, page, int8, window, sinks):
     """prompts and chunks of prompts, among them rows that stand for no token; rows of no sequence before and behind them"""
     run(Paged(rows, lens, Hkv, G, D, page, int8, extra=5, row0=1), window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("n,Hkv,G", [(65, 2, 4), (100, 1, 1), (700, 1, 20)])
+def test_prompts_of_many_sequences(n, Hkv, G, int8):
+    """more sequences than are put in order by what they see, and than a block looks at together; decode rows and prompts side by side, some without rows"""
+    rows = [0 if i % 11 == 5 else (1 if i % 3 else 20 + i % 40) for i in range(n)]
+    run(Paged(rows, [r + (i * 37) % 200 for i, r in enumerate(rows)], Hkv, G, 64, 16, int8, extra=1))
+
+
+@pytest.mark.parametrize("rows,lens,Hkv,G,D", [([2000], [2000], 1, 1, 128), ([300], [9000], 1, 2, 64), ([40], [20000], 2, 4, 128), ([129, 60], [5000, 7000], 1, 2, 128)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (3000, 40)])
+def test_long_contexts(rows, lens, Hkv, G, D, window, sinks):
+    """tiles whose blocks several CTAs share, and rings that go round many times"""
+    run(Paged(rows, lens, Hkv, G, D, 64), window=window, sinks=sinks)
 
 
 @pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
@@ -91,7 +106,8 @@ def test_rising_scores(rows, lens, window, int8):
 
 
 @pytest.mark.parametrize("rows,lens,window,sinks", [([1, 1], [400, 150], 0, 0), ([1, 1], [400, 150], 100, 5), ([9, 3], [300, 77], 30, 4), ([200, 140], [330, 140], 0, 0),
-                                                    ([300, 100], [700, 120], 50, 20)])
+                                                    ([300, 100], [700, 120], 50, 20),
+                                                    ([40], [6000], 0, 0), ([6, 2], [3000, 1000], 0, 0)])
 def test_values_that_are_no_numbers(rows, lens, window, sinks):
     """a NaN or an infinity in v reaches the rows that see its token, and no other row of the call; one in an invisible key reaches nobody"""
     c = Paged(rows, lens, 2, 4, 64, 16)
