@@ -216,7 +216,7 @@ __global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kern
     }
     unsigned char* ring = smem + SM::RING;
     const unsigned bars = smem_u32(smem + SM::BARS);
-    const unsigned bar_full = bars, bar_empty = bars + 8 * SLOTS, bar_s = bar_empty + 8 * SLOTS, bar_p = bar_s + 32, bar_v = bar_p + 32, bar_o = bar_v + 16, bar_q = bar_o + 16;   // bar_s, bar_p: [half of the block][tile]
+    const unsigned bar_full = bars, bar_empty = bars + 8 * SLOTS, bar_s = bar_empty + 8 * SLOTS, bar_p = bar_s + 32, bar_v = bar_p + 32, bar_o = bar_v + 16, bar_q = bar_o + 16, bar_turn = bar_q + 16;   // bar_s, bar_p: [half of the block][tile]
     volatile PromptMeta* meta = (volatile PromptMeta*)(smem + SM::META);
     volatile int* abort_flag = &abort_flag_word;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -228,7 +228,7 @@ __global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kern
         for (int w = 0; w < 2; w++) {
             mbar_init(bar_s + 8 * w, 1); mbar_init(bar_s + 16 + 8 * w, 1);
             mbar_init(bar_p + 8 * w, 4); mbar_init(bar_p + 16 + 8 * w, 4);
-            mbar_init(bar_v + 8 * w, 1); mbar_init(bar_o + 8 * w, 1); mbar_init(bar_q + 8 * w, 4);
+            mbar_init(bar_v + 8 * w, 1); mbar_init(bar_o + 8 * w, 1); mbar_init(bar_q + 8 * w, 4); mbar_init(bar_turn + 8 * w, 4);
         }
         abort_flag_word = 0;
         odd_value = 0;
@@ -303,6 +303,22 @@ __global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kern
         auto wait = [&](unsigned bar, unsigned parity) {
             if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) alive = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit));
         };
+        // Heads of 128: the two tiles begin their exponentials in turns (tile 0, tile 1, tile 0, ...); side by side, the unit that computes them would be busy
+        // while both need it and idle while both do the rest (3 sequences of up to 2048 rows: 191 us without, 182 with; with turns that are passed on at the end
+        // 189).  One turn for each half of a block, seen or not.  Not where that costs: heads of 64, 6000 rows with a window of 1000, 94 / 100; 8 bits, whose
+        // widening takes as long, no difference.
+        constexpr bool TURNS = D == 128 && !S8;
+        unsigned turn_phase = w == 1 ? 0 : 1;
+        auto take_turn = [&] {
+            if (TURNS && tiles == 2) wait(bar_turn + 8 * w, turn_phase);
+            turn_phase ^= 1;
+        };
+        auto pass_turn = [&] {
+            if (TURNS && tiles == 2) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bar_turn + 8 * (1 - w));
+            }
+        };
         for (int j = 0; j < n && w < tiles && alive; j++) {
             const volatile PromptMeta& mt = meta[j % PR_META];
 #pragma unroll 1
@@ -314,6 +330,9 @@ __global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kern
                 const unsigned facts = mt.facts;
                 if (!(facts & 256u << w)) {
                     if (lane == 0) mbar_arrive(bp);
+                    take_turn();
+                    if (!alive) break;
+                    pass_turn();
                     continue;
                 }
                 unsigned xa[32], xb[32];
@@ -391,7 +410,7 @@ __global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kern
                 // ---- probabilities of 32 columns, over columns of S that have been read ----
                 auto weigh = [&](const unsigned (&x)[32], int q, auto all) {
                     constexpr bool ALL = decltype(all)::value != 0;
-                    float y[32];
+                    unsigned pk[16];
 #pragma unroll
                     for (int e = 0; e < 32; e += 2) {
                         f32x2 f2 = c2;
@@ -399,38 +418,35 @@ __global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kern
                             const float f = mt.k[4 * h + 2 * q + (e >> 4)] * c;
                             f2 = pack2(f, f);
                         }
-                        unpack2(fma2(pack2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), f2, s2), y[e], y[e + 1]);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) {
-                        y[e] = exp2_approx(y[e]);
-                        y[e + 1] = exp2_approx(y[e + 1]);
-                        if (!ALL && !(seen[q] & (1u << e))) y[e] = 0.0f;
-                        if (!ALL && !(seen[q] & (2u << e))) y[e + 1] = 0.0f;
-                    }
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pack2(y[e], y[e + 1]));
-                    if constexpr (S8) {
-#pragma unroll
-                        for (int e = 0; e < 32; e += 2) {
+                        float y0, y1;
+                        unpack2(fma2(pack2(__uint_as_float(x[e]), __uint_as_float(x[e + 1])), f2, s2), y0, y1);
+                        y0 = exp2_approx(y0); y1 = exp2_approx(y1);
+                        if (!ALL) {
+                            if (!(seen[q] & (1u << e))) y0 = 0.0f;
+                            if (!(seen[q] & (2u << e))) y1 = 0.0f;
+                        }
+                        sum[(e >> 1) & 1] = add2(sum[(e >> 1) & 1], pack2(y0, y1));
+                        if constexpr (S8) {
                             const float f = mt.v[4 * h + 2 * q + (e >> 4)];
-                            unpack2(mul2(pack2(y[e], y[e + 1]), pack2(f, f)), y[e], y[e + 1]);
+                            unpack2(mul2(pack2(y0, y1), pack2(f, f)), y0, y1);
                             if (!ALL) {                              // (a masked token has no part in its page's factor, which may be NaN)
-                                if (!(seen[q] & (1u << e))) y[e] = 0.0f;
-                                if (!(seen[q] & (2u << e))) y[e + 1] = 0.0f;
+                                if (!(seen[q] & (1u << e))) y0 = 0.0f;
+                                if (!(seen[q] & (2u << e))) y1 = 0.0f;
                             }
                         }
+                        pk[e >> 1] = pack_bf16x2(y0, y1);
                     }
-                    unsigned pk[16];
-#pragma unroll
-                    for (int e = 0; e < 32; e += 2) pk[e >> 1] = pack_bf16x2(y[e], y[e + 1]);
                     tc_st16(ts + 16 * q, pk);
                 };
+                take_turn();
+                if (!alive) break;
                 if (whole) {
                     weigh(xa, 0, IntConst<1>());
+                    pass_turn();
                     weigh(xb, 1, IntConst<1>());
                 } else {
                     weigh(xa, 0, IntConst<0>());
+                    pass_turn();
                     weigh(xb, 1, IntConst<0>());
                 }
                 tc_wait_st();
