@@ -570,45 +570,76 @@ __global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kern
             const long long ts = a.c.token_stride, thread_off = r0 * ts + ch * 16;
             int pending = 0;                               // fills f - pending .. f - 1 are on their way by cp.async
             const unsigned thread_dst = smem_u32(ring) + (ch >> 3) * HALF + r0 * 128 + (((ch & 7) ^ (r0 & 7)) << 4);
+            const unsigned plain_facts = tiles == 2 ? 0x000f0300u : 0x00030100u;       // all rows see all of it, and its pages are there
+            int slot = 0;
+            unsigned phase = 0;
+            auto advance = [&] { if (++slot == SLOTS) { slot = 0; phase ^= 1; } };
             for (int j = 0; j < n && alive; j++) {
                 const int tok0 = block_token(j), page = next_page;
                 const unsigned bad = __ballot_sync(0xffffffffu, lane < 8 && page < 0) & 255u;
+                // Blocks that all rows see come by TMA, which one lane asks for: the four warps together took 650 clocks a fill, and were what a block waited for.
+                // The others come token by token, with zeros for those that nobody sees.
+                const bool plain = p.tma && bad == 0 && tok0 + 127 <= lo && (a.window == 0 || tok0 > hi - a.window || tok0 + 127 < a.sinks);
+                if (plain) {
+                    if (pending) {
+                        cp_async_wait<0>();
+                        for (; pending; pending--) arrived(2 * j - pending);
+                    }
+                    if (warp == PR_LOADER) {
+                        int pages[8];
+#pragma unroll
+                        for (int q = 0; q < 8; q++) pages[q] = __shfl_sync(0xffffffffu, page, (q << (psh - 4)) & 7);
+                        if (lane == 0) {
+                            meta[j % PR_META].tok0 = tok0;
+                            meta[j % PR_META].facts = plain_facts;
+                            int at = slot;
+                            unsigned ph = phase;
+#pragma unroll
+                            for (int kv = 0; kv < 2; kv++) {
+                                const unsigned full = bar_full + 8 * at, dst = smem_u32(ring) + at * SM::TILE;
+                                if (!mbar_wait(bar_empty + 8 * at, ph ^ 1, abort_flag, limit)) break;
+                                mbar_expect_tx(full, SM::TILE);
+#pragma unroll
+                                for (int q = 0; q < 8; q++)
+                                    if (q < 16 >> (psh - 3)) {
+#pragma unroll
+                                        for (int h = 0; h < D / 64; h++) tma_load_4d(dst + h * HALF + (q << (psh + 7)), kv ? &map_v : &map_k, full, 64 * h, 0, it.hk, pages[q]);
+                                    }
+                                if (++at == SLOTS) { at = 0; ph ^= 1; }
+                            }
+                        }
+                        __syncwarp();
+                        advance();
+                        advance();
+                    } else {
+                        // (the other warps take part in every fill: one that ran ahead or fell behind by a turn of the ring would wait for the wrong phase)
+                        if (lane == 0) {
+                            int at = slot;
+                            unsigned ph = phase;
+#pragma unroll
+                            for (int kv = 0; kv < 2; kv++) {
+                                if (!mbar_wait(bar_empty + 8 * at, ph ^ 1, abort_flag, limit)) break;
+                                mbar_arrive(bar_full + 8 * at);
+                                if (++at == SLOTS) { at = 0; ph ^= 1; }
+                            }
+                        }
+                        __syncwarp();
+                        advance();
+                        advance();
+                    }
+                    look_up(j + 1);
+                    continue;
+                }
                 if (tid == 0) {
                     meta[j % PR_META].tok0 = tok0;
                     meta[j % PR_META].facts = facts(tok0, bad);
                 }
                 look_up(j + 1);
-                // blocks that all rows see come by TMA, the others token by token with zeros for those that nobody sees
-                const bool plain = p.tma && bad == 0 && tok0 + 127 <= lo && (a.window == 0 || tok0 > hi - a.window || tok0 + 127 < a.sinks);
 #pragma unroll 1
                 for (int kv = 0; kv < 2; kv++) {
-                    const int f = 2 * j + kv, slot = f % SLOTS;
-                    alive = __all_sync(0xffffffffu, mbar_wait(bar_empty + 8 * slot, ((f / SLOTS) & 1) ^ 1, abort_flag, limit));
+                    const int f = 2 * j + kv;
+                    alive = __all_sync(0xffffffffu, mbar_wait(bar_empty + 8 * slot, phase ^ 1, abort_flag, limit));
                     if (!alive) break;
-                    if (plain) {
-                        if (pending) {
-                            cp_async_wait<0>();
-                            for (; pending; pending--) arrived(f - pending);
-                        }
-                        if (warp == PR_LOADER) {
-                            const unsigned full = bar_full + 8 * slot, dst = smem_u32(ring + slot * SM::TILE);
-                            const bool one = elect_one();
-                            if (one) mbar_expect_tx(full, SM::TILE);
-                            const int per = 16 >> (psh - 3);            // pages of a block
-#pragma unroll
-                            for (int q = 0; q < 8; q++) {
-                                const int pg = __shfl_sync(0xffffffffu, page, (q << (psh - 4)) & 7);
-                                if (q < per && one) {
-#pragma unroll
-                                    for (int h = 0; h < D / 64; h++) tma_load_4d(dst + h * HALF + (q << (psh + 7)), kv ? &map_v : &map_k, full, 64 * h, 0, it.hk, pg);
-                                }
-                            }
-                            __syncwarp();
-                        } else if (lane == 0) {
-                            mbar_arrive(bar_full + 8 * slot);
-                        }
-                        continue;
-                    }
                     const unsigned char* base = (kv ? a.c.v : a.c.k) + (long long)it.hk * a.c.head_stride;
                     const unsigned dst = thread_dst + slot * SM::TILE;
 #pragma unroll
@@ -623,6 +654,7 @@ __global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kern
                     }
                     cp_async_commit();
                     if (++pending > SM::AHEAD) { cp_async_wait<SM::AHEAD>(); arrived(f - SM::AHEAD); pending--; }
+                    advance();
                 }
             }
             cp_async_wait<0>();
