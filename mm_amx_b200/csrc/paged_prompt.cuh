@@ -103,6 +103,18 @@ __device__ __forceinline__ int over_group(const PromptParams& p, int n) {
     return q - (q * p.a.G > n);
 }
 
+// a packed row as row of the sequence and head of the group
+struct PackedRow {
+    int row, head;
+    __device__ __forceinline__ PackedRow(const PromptParams& p, int i) : row(over_group(p, i)), head(i - row * p.a.G) {}
+    __device__ __forceinline__ void advance(const PromptParams& p, int by) {      // (by: the same few numbers for all rows)
+        const int rows = over_group(p, by);
+        row += rows;
+        head += by - rows * p.a.G;
+        if (head >= p.a.G) { head -= p.a.G; row++; }
+    }
+};
+
 // A CTA's work: a tile of a (sequence, kv head) and a share of its blocks.
 struct PromptItem {
     int b, hk, row0;              // row0: first packed row
@@ -269,12 +281,14 @@ __global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kern
             constexpr int CH = D / 8, AT_ONCE = 128 / CH;
             const int r0 = tid / CH, ch = tid % CH;
             unsigned char* qt = smem + w * SM::TILE + (ch >> 3) * HALF;
+            PackedRow at(p, it.row0 + 128 * w + r0);
+            const unsigned char* q0 = a.q + (long long)it.s.row0 * a.q_rs + (long long)it.hk * a.G * a.q_hs + ch * 16;
 #pragma unroll
             for (int k = 0; k < CH; k++) {
-                const int r = k * AT_ONCE + r0, i = it.row0 + 128 * w + r, row = over_group(p, i);
+                const int r = k * AT_ONCE + r0;
                 const bool ok = 128 * w + r < it.rows;
-                cp_async16_or_zero(smem_u32(qt + r * 128 + (((ch & 7) ^ (r & 7)) << 4)),
-                                   ok ? a.q + (long long)(it.s.row0 + row) * a.q_rs + (long long)(it.hk * a.G + i - row * a.G) * a.q_hs + ch * 16 : a.q, ok);
+                cp_async16_or_zero(smem_u32(qt + r * 128 + (((ch & 7) ^ (r & 7)) << 4)), ok ? q0 + at.row * a.q_rs + at.head * a.q_hs : a.q, ok);
+                at.advance(p, AT_ONCE);
             }
             cp_async_commit();
             cp_async_wait<0>();
@@ -494,12 +508,14 @@ __global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kern
             }
             if (!split) {
                 __syncwarp();
+                const int ch = lane % CH, i2 = 128 * w + (warp & 3) * 32 + lane / CH;
+                PackedRow at(p, it.row0 + i2);
+                unsigned char* out0 = a.out + (long long)it.s.row0 * a.o_rs + (long long)it.hk * a.G * a.o_hs + ch * 16;
 #pragma unroll
                 for (int k = 0; k < CH; k++) {
-                    const int r = k * AT_ONCE + lane / CH, ch = lane % CH, i2 = 128 * w + (warp & 3) * 32 + r, row2 = over_group(p, it.row0 + i2);
-                    if (i2 < it.rows)
-                        *(uint4*)(a.out + (long long)(it.s.row0 + row2) * a.o_rs + (long long)(it.hk * a.G + it.row0 + i2 - row2 * a.G) * a.o_hs + ch * 16) =
-                            *(const uint4*)(own + r * D * 2 + ((ch ^ (r & 7)) << 4));
+                    const int r = k * AT_ONCE + lane / CH;
+                    if (i2 + k * AT_ONCE < it.rows) *(uint4*)(out0 + at.row * a.o_rs + at.head * a.o_hs) = *(const uint4*)(own + r * D * 2 + ((ch ^ (r & 7)) << 4));
+                    at.advance(p, AT_ONCE);
                 }
             }
             if (split && mine) *(float2*)(p.ws_ml + ((size_t)blockIdx.x * PR_ROWS + i) * 2) = make_float2(m_used, l);
