@@ -22,6 +22,7 @@ namespace {
 
 constexpr int PR_ROWS = 256, PR_BLOCK = 128;       // packed rows of a CTA, tokens of a block
 constexpr int PR_LOADER = 8;                       // first of the warps that fetch
+constexpr int PR_FIND_BYTES = 1024;
 constexpr int PR_META = 8;                         // blocks whose facts are kept; more than the ring holds
 
 // Warps and registers.  8 bits are widened by eight warps (with four they were the bottleneck: 185 us where this takes 155), bf16 needs four.  The last two warps
@@ -40,8 +41,8 @@ template <int D> struct PromptSmem {
     static constexpr int AHEAD = D == 128 ? 2 : 3;                    // fetched blocks whose arrival is waited for later
     static constexpr int RING = 2 * TILE, BARS = RING + SLOTS * TILE;
     static constexpr int META = BARS + 384;
-    static constexpr int ROWS = META + PR_META * 80;                  // what a row's two threads tell one another; before that, the search for the tile
-    static constexpr int BYTES = ROWS + 2 * 128 * 2 * 4;              // (D = 128: all there is)
+    static constexpr int FIND = META + PR_META * 80;                  // for the search for the tile
+    static constexpr int BYTES = FIND + PR_FIND_BYTES;
     static_assert(BYTES <= 232448, "shared memory of a CTA");
 };
 // Of a block: its first token; granules of 16 tokens that lie in no page of the pool (bits 0-7), whether tile w sees any of it (bit 8 + w) and all rows of the
@@ -103,18 +104,6 @@ __device__ __forceinline__ int over_group(const PromptParams& p, int n) {
     return q - (q * p.a.G > n);
 }
 
-// a packed row as row of the sequence and head of the group
-struct PackedRow {
-    int row, head;
-    __device__ __forceinline__ PackedRow(const PromptParams& p, int i) : row(over_group(p, i)), head(i - row * p.a.G) {}
-    __device__ __forceinline__ void advance(const PromptParams& p, int by) {      // (by: the same few numbers for all rows)
-        const int rows = over_group(p, by);
-        row += rows;
-        head += by - rows * p.a.G;
-        if (head >= p.a.G) { head -= p.a.G; row++; }
-    }
-};
-
 // A CTA's work: a tile of a (sequence, kv head) and a share of its blocks.
 struct PromptItem {
     int b, hk, row0;              // row0: first packed row
@@ -131,7 +120,7 @@ struct FindSpace {
     PromptItem item;
     int warp_sum[PromptShape<true>::THREADS / 32], keys[PR_RANKED], order[PR_RANKED];
 };
-static_assert(sizeof(FindSpace) <= 2048, "lies where the rows' values come later");
+static_assert(sizeof(FindSpace) <= PR_FIND_BYTES, "");
 template <int THREADS>
 __device__ __forceinline__ bool find_prompt_item(const PagedAttn& a, int item, int split, int splits, bool report, PromptItem* it, FindSpace* space) {
     PromptItem* shared = &space->item;
@@ -221,7 +210,6 @@ __global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kern
     int& odd_value = *(int*)(smem + SM::BARS + 368);
     int& abort_flag_word = *(int*)(smem + SM::BARS + 372);
     unsigned& tmem_holder = *(unsigned*)(smem + SM::BARS + 376);
-    float* row_values = (float*)(smem + SM::ROWS);
     if (smem_u32(smem) & 1023u) {
         if (threadIdx.x == 0) atomicExch(p.a.c.status, 4);
         return;
@@ -252,7 +240,7 @@ __global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kern
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     PromptItem it;
-    const bool has_item = find_prompt_item<PR_THREADS>(a, (int)(blockIdx.x / p.splits), (int)(blockIdx.x % p.splits), p.splits, blockIdx.x == 0, &it, (FindSpace*)row_values);
+    const bool has_item = find_prompt_item<PR_THREADS>(a, (int)(blockIdx.x / p.splits), (int)(blockIdx.x % p.splits), p.splits, blockIdx.x == 0, &it, (FindSpace*)(smem + SM::FIND));
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -281,14 +269,12 @@ __global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kern
             constexpr int CH = D / 8, AT_ONCE = 128 / CH;
             const int r0 = tid / CH, ch = tid % CH;
             unsigned char* qt = smem + w * SM::TILE + (ch >> 3) * HALF;
-            PackedRow at(p, it.row0 + 128 * w + r0);
-            const unsigned char* q0 = a.q + (long long)it.s.row0 * a.q_rs + (long long)it.hk * a.G * a.q_hs + ch * 16;
 #pragma unroll
             for (int k = 0; k < CH; k++) {
-                const int r = k * AT_ONCE + r0;
+                const int r = k * AT_ONCE + r0, i = it.row0 + 128 * w + r, row = over_group(p, i);
                 const bool ok = 128 * w + r < it.rows;
-                cp_async16_or_zero(smem_u32(qt + r * 128 + (((ch & 7) ^ (r & 7)) << 4)), ok ? q0 + at.row * a.q_rs + at.head * a.q_hs : a.q, ok);
-                at.advance(p, AT_ONCE);
+                cp_async16_or_zero(smem_u32(qt + r * 128 + (((ch & 7) ^ (r & 7)) << 4)),
+                                   ok ? a.q + (long long)(it.s.row0 + row) * a.q_rs + (long long)(it.hk * a.G + i - row * a.G) * a.q_hs + ch * 16 : a.q, ok);
             }
             cp_async_commit();
             cp_async_wait<0>();
@@ -508,14 +494,12 @@ __global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kern
             }
             if (!split) {
                 __syncwarp();
-                const int ch = lane % CH, i2 = 128 * w + (warp & 3) * 32 + lane / CH;
-                PackedRow at(p, it.row0 + i2);
-                unsigned char* out0 = a.out + (long long)it.s.row0 * a.o_rs + (long long)it.hk * a.G * a.o_hs + ch * 16;
 #pragma unroll
                 for (int k = 0; k < CH; k++) {
-                    const int r = k * AT_ONCE + lane / CH;
-                    if (i2 + k * AT_ONCE < it.rows) *(uint4*)(out0 + at.row * a.o_rs + at.head * a.o_hs) = *(const uint4*)(own + r * D * 2 + ((ch ^ (r & 7)) << 4));
-                    at.advance(p, AT_ONCE);
+                    const int r = k * AT_ONCE + lane / CH, ch = lane % CH, i2 = 128 * w + (warp & 3) * 32 + r, row2 = over_group(p, it.row0 + i2);
+                    if (i2 < it.rows)
+                        *(uint4*)(a.out + (long long)(it.s.row0 + row2) * a.o_rs + (long long)(it.hk * a.G + it.row0 + i2 - row2 * a.G) * a.o_hs + ch * 16) =
+                            *(const uint4*)(own + r * D * 2 + ((ch ^ (r & 7)) << 4));
                 }
             }
             if (split && mine) *(float2*)(p.ws_ml + ((size_t)blockIdx.x * PR_ROWS + i) * 2) = make_float2(m_used, l);
@@ -586,76 +570,45 @@ __global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kern
             const long long ts = a.c.token_stride, thread_off = r0 * ts + ch * 16;
             int pending = 0;                               // fills f - pending .. f - 1 are on their way by cp.async
             const unsigned thread_dst = smem_u32(ring) + (ch >> 3) * HALF + r0 * 128 + (((ch & 7) ^ (r0 & 7)) << 4);
-            const unsigned plain_facts = tiles == 2 ? 0x000f0300u : 0x00030100u;       // all rows see all of it, and its pages are there
-            int slot = 0;
-            unsigned phase = 0;
-            auto advance = [&] { if (++slot == SLOTS) { slot = 0; phase ^= 1; } };
             for (int j = 0; j < n && alive; j++) {
                 const int tok0 = block_token(j), page = next_page;
                 const unsigned bad = __ballot_sync(0xffffffffu, lane < 8 && page < 0) & 255u;
-                // Blocks that all rows see come by TMA, which one lane asks for: the four warps together took 650 clocks a fill, and were what a block waited for.
-                // The others come token by token, with zeros for those that nobody sees.
-                const bool plain = p.tma && bad == 0 && tok0 + 127 <= lo && (a.window == 0 || tok0 > hi - a.window || tok0 + 127 < a.sinks);
-                if (plain) {
-                    if (pending) {
-                        cp_async_wait<0>();
-                        for (; pending; pending--) arrived(2 * j - pending);
-                    }
-                    if (warp == PR_LOADER) {
-                        int pages[8];
-#pragma unroll
-                        for (int q = 0; q < 8; q++) pages[q] = __shfl_sync(0xffffffffu, page, (q << (psh - 4)) & 7);
-                        if (lane == 0) {
-                            meta[j % PR_META].tok0 = tok0;
-                            meta[j % PR_META].facts = plain_facts;
-                            int at = slot;
-                            unsigned ph = phase;
-#pragma unroll
-                            for (int kv = 0; kv < 2; kv++) {
-                                const unsigned full = bar_full + 8 * at, dst = smem_u32(ring) + at * SM::TILE;
-                                if (!mbar_wait(bar_empty + 8 * at, ph ^ 1, abort_flag, limit)) break;
-                                mbar_expect_tx(full, SM::TILE);
-#pragma unroll
-                                for (int q = 0; q < 8; q++)
-                                    if (q < 16 >> (psh - 3)) {
-#pragma unroll
-                                        for (int h = 0; h < D / 64; h++) tma_load_4d(dst + h * HALF + (q << (psh + 7)), kv ? &map_v : &map_k, full, 64 * h, 0, it.hk, pages[q]);
-                                    }
-                                if (++at == SLOTS) { at = 0; ph ^= 1; }
-                            }
-                        }
-                        __syncwarp();
-                        advance();
-                        advance();
-                    } else {
-                        // (the other warps take part in every fill: one that ran ahead or fell behind by a turn of the ring would wait for the wrong phase)
-                        if (lane == 0) {
-                            int at = slot;
-                            unsigned ph = phase;
-#pragma unroll
-                            for (int kv = 0; kv < 2; kv++) {
-                                if (!mbar_wait(bar_empty + 8 * at, ph ^ 1, abort_flag, limit)) break;
-                                mbar_arrive(bar_full + 8 * at);
-                                if (++at == SLOTS) { at = 0; ph ^= 1; }
-                            }
-                        }
-                        __syncwarp();
-                        advance();
-                        advance();
-                    }
-                    look_up(j + 1);
-                    continue;
-                }
                 if (tid == 0) {
                     meta[j % PR_META].tok0 = tok0;
                     meta[j % PR_META].facts = facts(tok0, bad);
                 }
                 look_up(j + 1);
+                // blocks that all rows see come by TMA, the others token by token with zeros for those that nobody sees
+                const bool plain = p.tma && bad == 0 && tok0 + 127 <= lo && (a.window == 0 || tok0 > hi - a.window || tok0 + 127 < a.sinks);
 #pragma unroll 1
                 for (int kv = 0; kv < 2; kv++) {
-                    const int f = 2 * j + kv;
-                    alive = __all_sync(0xffffffffu, mbar_wait(bar_empty + 8 * slot, phase ^ 1, abort_flag, limit));
+                    const int f = 2 * j + kv, slot = f % SLOTS;
+                    alive = __all_sync(0xffffffffu, mbar_wait(bar_empty + 8 * slot, ((f / SLOTS) & 1) ^ 1, abort_flag, limit));
                     if (!alive) break;
+                    if (plain) {
+                        if (pending) {
+                            cp_async_wait<0>();
+                            for (; pending; pending--) arrived(f - pending);
+                        }
+                        if (warp == PR_LOADER) {
+                            const unsigned full = bar_full + 8 * slot, dst = smem_u32(ring + slot * SM::TILE);
+                            const bool one = elect_one();
+                            if (one) mbar_expect_tx(full, SM::TILE);
+                            const int per = 16 >> (psh - 3);            // pages of a block
+#pragma unroll
+                            for (int q = 0; q < 8; q++) {
+                                const int pg = __shfl_sync(0xffffffffu, page, (q << (psh - 4)) & 7);
+                                if (q < per && one) {
+#pragma unroll
+                                    for (int h = 0; h < D / 64; h++) tma_load_4d(dst + h * HALF + (q << (psh + 7)), kv ? &map_v : &map_k, full, 64 * h, 0, it.hk, pg);
+                                }
+                            }
+                            __syncwarp();
+                        } else if (lane == 0) {
+                            mbar_arrive(bar_full + 8 * slot);
+                        }
+                        continue;
+                    }
                     const unsigned char* base = (kv ? a.c.v : a.c.k) + (long long)it.hk * a.c.head_stride;
                     const unsigned dst = thread_dst + slot * SM::TILE;
 #pragma unroll
@@ -670,7 +623,6 @@ __global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kern
                     }
                     cp_async_commit();
                     if (++pending > SM::AHEAD) { cp_async_wait<SM::AHEAD>(); arrived(f - SM::AHEAD); pending--; }
-                    advance();
                 }
             }
             cp_async_wait<0>();
