@@ -562,7 +562,7 @@ int launch_paged_decode_as(DecParams& p, cudaStream_t s) {
     p.prefix = (long long*)(p.ws_ml + states * 2);
     cudaLaunchAttribute attr[1];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = getenv("X_NOPDL") ? 0 : 1;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)p.ctas);
     cfg.blockDim = dim3(DEC_THREADS);
