@@ -106,7 +106,7 @@ int check_kernel_status(cudaStream_t s, int* pinned = nullptr);  // synchronises
 // growing device scratch owned by (device, stream, slot): work on one stream is ordered, so kernels launched on it
 // may share it; slot 0 = re-strided activations, slot 1 = split-K partial tiles of the GEMM and sums of folded parts of K, 3 = widened weight
 // rows, 4 = normalised activations of the MLP block, 5 = sub-states of the decode attention, 6 = pre-converted activations
-// of the decode kernel
+// of the decode kernel, 7 / 8 = sub-states of the paged attention (few rows / prompts)
 // own (optional): where s is being captured, stream-ordered memory instead, which becomes part of the graph (the stream's scratch may be
 // re-allocated before a replay); *own says so, and the caller frees it with cudaFreeAsync behind its last use
 int get_stream_scratch(size_t bytes, cudaStream_t s, int slot, void** out, bool* own = nullptr);

@@ -61,7 +61,7 @@ def test_prompts(rows, lens, Hkv, G, D, page, int8, window, sinks):
 
 
 @pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
-@pytest.mark.parametrize("n,Hkv,G", [(32, 2, 4), (33, 2, 4), (100, 1, 1), (1000, 1, 20)])
+@pytest.mark.parametrize("n,Hkv,G", [(32, 2, 4), (33, 2, 4), (64, 2, 4), (65, 2, 4), (100, 1, 1), (1000, 1, 20)])
 def test_prompts_of_many_sequences(n, Hkv, G, int8):
     """more sequences than are put in order by what they see, and than a block looks at together; decode rows and prompts side by side, some without rows"""
     rows = [0 if i % 11 == 5 else (1 if i % 3 else 20 + i % 40) for i in range(n)]
