@@ -319,7 +319,7 @@ typedef struct {
  *   int8       a page's factor is s = max(s of the tokens it holds already, largest new |value| / 127), new values are stored as rne(x / s), and where s
  *              grew the older ones as rne(q * s_before / s), with fp32 products by 1 / s; a factor below 2^-126 is stored as 0.  A page of which the call
  *              writes place 0 starts anew.  A page that holds or receives an infinity or a NaN has the factor NaN from then on.
- * Two sequences of a call may share pages only where neither writes.  q NULL: none; q_out may be q itself (with q's strides), no other overlap.
+ * Two sequences of a call may share pages only where neither writes, and a page that is written stands in its row of the table once.  q NULL: none; q_out may be q itself (with q's strides), no other overlap.
  * rot_dim: a multiple of 16, at most D.  q, k, v, q_out, rot_cos, rot_sin and their strides 16-byte aligned. */
 typedef struct {
     const b200fc_paged_cache_t* cache;
@@ -341,7 +341,8 @@ int b200fc_kv_append(const b200fc_kv_append_t* a, void* stream);
 /* out[r, h, :] = sum_j softmax_j(scale * q[r, h, :] . k_j) v_j over the cached tokens j of the row's sequence that are visible to its place p:
  * j <= p, and with window > 0 only the last `window` of them (j > p - window) and the first `sinks` tokens of the sequence (j < sinks).  Rows that see no
  * token are zeros.  Scores, softmax and sums are fp32; probabilities are rounded to bf16 for the product with v.  H / Hkv query heads share a kv head
- * (any number).  max_rows, at least 1: no sequence has more rows (a sequence that has is left out, as above).  q and out bf16, 16-byte aligned with their strides.
+ * (any number).  max_rows, at least 1: no sequence has more rows (a sequence that has is left out, as above).  q and out bf16, 16-byte aligned with their strides; out overlaps
+ * neither q nor the cache.
  * What lies behind a sequence's last token, or is invisible to all its rows, may be anything, NaN included.  k and v of visible tokens: any bf16. */
 typedef struct {
     const b200fc_paged_cache_t* cache;
