@@ -1,6 +1,7 @@
 // Attention over the paged cache: checks of the call and the choice of its kernel.
 #include <algorithm>
 #include <cfloat>
+#include <cmath>
 #include "paged_common.cuh"
 #include "paged_decode.cuh"
 #include "paged_prompt.cuh"
@@ -20,6 +21,7 @@ int launch_paged_attention(const b200fc_paged_attention_t& a, cudaStream_t s) {
     }
     // (rows that met a value that is no number are done again from q, when some of out is written)
     if (a.out == a.q) { set_error("paged_attention: out must not be q"); return B200FC_ERR_INVALID; }
+    if (!std::isfinite(a.scale)) { set_error("paged_attention: scale is no number"); return B200FC_ERR_INVALID; }
     if (a.window < 0 || a.sinks < 0) { set_error("paged_attention: negative window or sinks"); return B200FC_ERR_INVALID; }
     if (a.T == 0 || c.B == 0) return B200FC_OK;
     if (a.max_rows < 1) { set_error("paged_attention: max_rows must be at least 1"); return B200FC_ERR_INVALID; }
