@@ -21,7 +21,8 @@ int launch_paged_attention(const b200fc_paged_attention_t& a, cudaStream_t s) {
     }
     // (rows that met a value that is no number are done again from q, when some of out is written)
     if (a.out == a.q) { set_error("paged_attention: out must not be q"); return B200FC_ERR_INVALID; }
-    if (!std::isfinite(a.scale)) { set_error("paged_attention: scale is no number"); return B200FC_ERR_INVALID; }
+    p.scale_log2e = a.scale * 1.4426950408889634f;
+    if (!std::isfinite(p.scale_log2e)) { set_error("paged_attention: scale is no number, or 2^127 and more"); return B200FC_ERR_INVALID; }
     if (a.window < 0 || a.sinks < 0) { set_error("paged_attention: negative window or sinks"); return B200FC_ERR_INVALID; }
     if (a.T == 0 || c.B == 0) return B200FC_OK;
     if (a.max_rows < 1) { set_error("paged_attention: max_rows must be at least 1"); return B200FC_ERR_INVALID; }
@@ -32,7 +33,6 @@ int launch_paged_attention(const b200fc_paged_attention_t& a, cudaStream_t s) {
     p.H = a.H; p.G = a.H / c.Hkv;
     p.window = a.window < p.c.capacity ? a.window : 0;        // (a window as long as the cache is none)
     p.sinks = a.sinks;
-    p.scale_log2e = a.scale * 1.4426950408889634f;
     const bool s8 = c.dtype == B200FC_S8;
     p.c.max_rows = a.row_start ? std::min(a.max_rows, a.T) : 1;
     if ((long long)p.c.max_rows * p.G <= 16 && (long long)c.B * c.Hkv < (1LL << 31)) {

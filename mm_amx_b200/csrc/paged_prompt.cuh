@@ -577,6 +577,7 @@ __global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kern
                     meta[j % PR_META].tok0 = tok0;
                     meta[j % PR_META].facts = facts(tok0, bad);
                 }
+                __syncwarp();                              // (another lane may be the one that announces the block)
                 look_up(j + 1);
                 // blocks that all rows see come by TMA, the others token by token with zeros for those that nobody sees
                 const bool plain = p.tma && bad == 0 && tok0 + 127 <= lo && (a.window == 0 || tok0 > hi - a.window || tok0 + 127 < a.sinks);

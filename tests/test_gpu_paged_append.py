@@ -154,6 +154,16 @@ def test_layouts(layout, int8):
     check_append(c, 64, False, turns=tables(100, 64, 8))
 
 
+@pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
+def test_sequences_that_share_pages_none_writes(int8):
+    """what several sequences begin with stays as it is"""
+    c = Paged([20, 1, 33], [90, 81, 97], 2, 2, 64, 16, int8)
+    for b in (1, 2):
+        c.ids[b][:4] = c.ids[0][:4]
+        c.table[b, :4] = c.table[0, :4]
+    check_append(c)
+
+
 def test_factors_that_grow_and_stay():
     """new values smaller than a page's, larger, all zero, and values whose factor is too small for fp32"""
     for std in (0.0, 1e-3, 1.0, 50.0, 1e-39):

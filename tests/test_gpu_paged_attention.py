@@ -125,6 +125,32 @@ def test_values_that_are_no_numbers(rows, lens, window, sinks):
     run(c, window=window, sinks=sinks)
 
 
+@pytest.mark.parametrize("rows,lens", [([1, 1], [400, 150]), ([3, 4], [300, 77]), ([200, 140], [330, 140]), ([40, 30], [6000, 100])])
+def test_rows_of_q_that_are_no_numbers(rows, lens):
+    """a NaN in q stays with its row and head"""
+    c = Paged(rows, lens, 2, 4, 128, 16)
+    hit = [(0, 1), (rows[0] - 1, 6), (c.T - 1, 2)]
+    want, mag = c.attended()
+    for r, h in hit:
+        c.q[r, h, 77] = float("nan")
+        want[r, h] = float("nan")
+    got = c.attend()
+    capi.sync_check()
+    c.check(got, want, mag)
+
+
+@pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("rows", [[1, 1, 1], [2, 3, 1], [60, 200, 1]], ids=str)
+def test_sequences_that_share_their_first_pages(rows, int8):
+    """what several sequences begin with stands in the cache once"""
+    c = Paged(rows, [320, 300, 129], 2, 4, 64, 16, int8)
+    for b in (1, 2):
+        c.ids[b][:5] = c.ids[0][:5]
+        c.table[b, :5] = c.table[0, :5]
+    run(c)
+    run(c, window=250, sinks=3)
+
+
 def test_pages_that_no_row_sees_are_not_read():
     """pages behind the window may have been given back: their entries name other pages, or none"""
     for rows, lens in (([1, 1], [1000, 300]), ([40], [900])):

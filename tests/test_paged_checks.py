@@ -47,7 +47,7 @@ BAD_APPEND = [dict(k=None), dict(v=None), dict(q_out=None), dict(H=0), dict(H=-1
               dict(axes=3, section=(capi.c_int * 3)(16, 8, 8), positions=A, position_stride=4), dict(row_start=A + 1)]
 BAD_ATTEND = [dict(q=None), dict(out=None), dict(H=0), dict(H=3), dict(H=70000), dict(T=-1), dict(max_rows=-1), dict(max_rows=0), dict(q=A + 8), dict(out=A + 2), dict(q_row_stride=520),
               dict(out_head_stride=8), dict(window=-1), dict(sinks=-1), dict(row_start=A + 2), dict(T=1), dict(T=3), dict(out=A),
-              dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=-float("inf"))]
+              dict(scale=float("nan")), dict(scale=float("inf")), dict(scale=-float("inf")), dict(scale=3e38)]
 
 
 def refused(call, *args, **kw):
