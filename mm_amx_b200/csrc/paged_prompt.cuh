@@ -3,12 +3,15 @@
 //
 // A CTA takes 256 packed rows of one (sequence, kv head), as two tiles of 128 rows, over all 128-token blocks that they see, or over a share of those
 // where the call has too few tiles for the GPU.  Packing the heads of a group into the rows keeps K and V of a block in shared memory for all of them.
+// With heads of 64 in bf16 a CTA takes one tile, and an SM two CTAs: what a CTA does before its first block and after its last (7 us) then runs under the
+// other's blocks, and the last tiles are shorter (6000 rows, window 1000, 16 heads: 94 us with two tiles, 83 with one; 2 x up to 2048 rows, 4096 tokens, 16
+// heads: 78 / 62).  Heads of 128 have no room for that in shared memory, and 8 bits would be widened twice.
 //   warps 0-3, 4-7   softmax of tile 0, 1: a thread has one row.  S comes from tensor memory 64 tokens at a time, exp2(S - max) goes back over it as bf16.  The
 //                    maximum that is subtracted follows the true one only when that is 2^8 ahead (sums and values are fp32 and stay far from their limits, the
 //                    probabilities' rounding is relative), so that O in tensor memory is rescaled hardly ever.
-//   4 or 8 more      fetch K and V blocks into a ring of 128-token slots (128-byte swizzle): bf16 by TMA, or in blocks that not every row sees by cp.async with zeros
+//   2, 4 or 8 more   fetch K and V blocks into a ring of 128-token slots (128-byte swizzle): bf16 by TMA, or in blocks that not every row sees by cp.async with zeros
 //                    for tokens that nobody sees (which may hold anything), 8 bits widened on the way to bf16 of (value / 64), exactly; the page's factors go to the softmax.
-//   two more         issue the products of tile 0, 1: S_w = Q_w K^T (Q, K in shared memory), O_w += P_w V (P in tensor memory, V as it lies: N-major).  One
+//   one a tile       issues its products: S_w = Q_w K^T (Q, K in shared memory), O_w += P_w V (P in tensor memory, V as it lies: N-major).  One
 //                    tile's products run under the other tile's softmax.  (One warp for both tiles was the bottleneck: 3900 clocks a block.)
 // Tensor memory: S_0 S_1 (128 columns each; P over the first half of either 64) O_0 O_1 (D columns each).
 // A value that is no number in a block that some rows do not see would reach them as 0 * NaN: the fetching warps look for one in such blocks, and a CTA that
@@ -20,30 +23,34 @@ namespace b200fc {
 
 namespace {
 
-constexpr int PR_ROWS = 256, PR_BLOCK = 128;       // packed rows of a CTA, tokens of a block
-constexpr int PR_LOADER = 8;                       // first of the warps that fetch
+constexpr int PR_BLOCK = 128;                      // tokens of a block
 constexpr int PR_FIND_BYTES = 1024;
 constexpr int PR_META = 8;                         // blocks whose facts are kept; more than the ring holds
 
-// Warps and registers.  8 bits are widened by eight warps (with four they were the bottleneck: 185 us where this takes 155), bf16 needs four.  The last two warps
-// only fill their group of four.
-template <bool S8> struct PromptShape {
-    static constexpr int MMA = PR_LOADER + (S8 ? 8 : 4), THREADS = (MMA + 4) * 32;
-    static constexpr int REGS = S8 ? 96 : 128, REGS_SOFTMAX = 152, REGS_OTHER = S8 ? 56 : 104;      // a thread, at launch and in the roles
-    static_assert(REGS_SOFTMAX * PR_LOADER * 32 + REGS_OTHER * (THREADS - PR_LOADER * 32) <= REGS * THREADS && REGS * THREADS <= 65536,
+// Warps and registers.  8 bits are widened by eight warps (with four they were the bottleneck: 185 us where this takes 155), bf16 needs two a tile.  The last
+// warps only fill their group of four.  (bf16, one tile: with 152 and 104 registers some are spilled, 90 us where this takes 83.)
+template <int D, bool S8> struct PromptShape {
+    static constexpr int TILES = D == 64 && !S8 ? 1 : 2, ROWS = 128 * TILES, CTAS = 3 - TILES;      // CTAs: per SM
+    static constexpr int LOADER = 4 * TILES, MMA = LOADER + (S8 ? 8 : 2 * TILES), THREADS = (MMA + 2 * TILES) * 32;      // first of the warps that fetch, that multiply
+    static constexpr int REGS = S8 ? 96 : 128, REGS_SOFTMAX = S8 ? 152 : 160, REGS_OTHER = S8 ? 56 : 96;      // a thread, at launch and in the roles
+    static constexpr int COLUMNS = 256 * TILES, O_AT = 128 * TILES;                                 // of tensor memory
+    static_assert(REGS_SOFTMAX * LOADER * 32 + REGS_OTHER * (THREADS - LOADER * 32) <= REGS * THREADS && REGS * THREADS * CTAS <= 65536,
                   "the split must not ask for more than the launch has");
+    static_assert(LOADER % 4 == 0 && (THREADS / 32) % 4 == 0, "registers are split between groups of four warps");
 };
 
-template <int D> struct PromptSmem {
+template <int D, bool S8> struct PromptSmem {
+    static constexpr int TILES = PromptShape<D, S8>::TILES;
     static constexpr int HALF = PR_BLOCK * 128;                       // 128 rows of 64 components
     static constexpr int TILE = HALF * (D / 64);                      // a tile of Q, a block of K or V
-    static constexpr int SLOTS = D == 128 ? 5 : 8;
-    static constexpr int AHEAD = D == 128 ? 2 : 3;                    // fetched blocks whose arrival is waited for later
-    static constexpr int RING = 2 * TILE, BARS = RING + SLOTS * TILE;
+    static constexpr int SLOTS = D == 128 || TILES == 1 ? 5 : 8;
+    static constexpr int AHEAD = SLOTS == 5 ? 2 : 3;                     // fetched blocks whose arrival is waited for later
+    static constexpr int RING = TILES * TILE, BARS = RING + SLOTS * TILE;
     static constexpr int META = BARS + 384;
     static constexpr int FIND = META + PR_META * 80;                  // for the search for the tile
     static constexpr int BYTES = FIND + PR_FIND_BYTES;
-    static_assert(BYTES <= 232448, "shared memory of a CTA");
+    static_assert(PromptShape<D, S8>::CTAS * (BYTES + 1024) <= 233472, "shared memory of the CTAs of an SM (1 KB of each is the system's)");
+    static_assert(BYTES % 1024 == 0 || PromptShape<D, S8>::CTAS == 1, "the swizzle goes by addresses: each CTA begins at a multiple of 1024");
 };
 // Of a block: its first token; granules of 16 tokens that lie in no page of the pool (bits 0-7), whether tile w sees any of it (bit 8 + w) and all rows of the
 // tile all of half h (bit 16 + 2 w + h); factors times 64.  Worked out once, by the warps that fetch it.
@@ -55,8 +62,8 @@ struct PromptParams {
     unsigned group_inverse;       // ceil(2^32 / G)
     unsigned flip;                // sign bits of two bf16: the scale's sign, carried by Q
     int splits;                   // CTAs that share a tile's blocks at most
-    float* ws_o;                  // [CTA][PR_ROWS][D]
-    float* ws_ml;                 // [CTA][PR_ROWS][2]
+    float* ws_o;                  // [CTA][ROWS][D]
+    float* ws_ml;                 // [CTA][ROWS][2]
     int tma;                      // the tensor maps are there
     unsigned long long wait_limit_ns;
 };
@@ -118,10 +125,10 @@ __device__ __forceinline__ int prompt_splits(int count, int splits) { return max
 constexpr int PR_RANKED = 64;
 struct FindSpace {
     PromptItem item;
-    int warp_sum[PromptShape<true>::THREADS / 32], keys[PR_RANKED], order[PR_RANKED];
+    int warp_sum[PromptShape<128, true>::THREADS / 32], keys[PR_RANKED], order[PR_RANKED];
 };
 static_assert(sizeof(FindSpace) <= PR_FIND_BYTES, "");
-template <int THREADS>
+template <int ROWS, int THREADS>
 __device__ __forceinline__ bool find_prompt_item(const PagedAttn& a, int item, int split, int splits, bool report, PromptItem* it, FindSpace* space) {
     PromptItem* shared = &space->item;
     int *warp_sum = space->warp_sum, *keys = space->keys, *order = space->order;
@@ -129,14 +136,14 @@ __device__ __forceinline__ bool find_prompt_item(const PagedAttn& a, int item, i
     auto sequence = [&](int b, SeqRows* s, int* tiles) {
         *s = SeqRows{0, 0, 0};
         const bool ok = load_seq(a.c, b, s);
-        *tiles = (s->rows * a.G + PR_ROWS - 1) / PR_ROWS;
+        *tiles = (s->rows * a.G + ROWS - 1) / ROWS;
         return ok;
     };
     auto found = [&](int b, const SeqRows& s, int tiles, int at) {
         const int rt = tiles - 1 - at / a.c.Hkv, first = s.len - s.rows;
         PromptItem x;
-        x.b = b; x.hk = at % a.c.Hkv; x.row0 = rt * PR_ROWS; x.s = s;
-        x.rows = min(PR_ROWS, s.rows * a.G - x.row0);
+        x.b = b; x.hk = at % a.c.Hkv; x.row0 = rt * ROWS; x.s = s;
+        x.rows = min(ROWS, s.rows * a.G - x.row0);
         x.kb = key_blocks(max(first + x.row0 / a.G, 0), first + (x.row0 + x.rows - 1) / a.G, a.window, a.sinks, 7);
         x.splits = prompt_splits(x.kb.count, splits);
         x.n0 = split < x.splits ? (int)((long long)x.kb.count * split / x.splits) : 0;
@@ -151,7 +158,7 @@ __device__ __forceinline__ bool find_prompt_item(const PagedAttn& a, int item, i
         if (b < a.c.B) {
             if (!sequence(b, &s, &tiles) && report) report_paged(a.c);
             n = tiles * a.c.Hkv;
-            const KeyBlocks kb = key_blocks(max(s.len - 1 - (PR_ROWS - 1) / a.G, 0), s.len - 1, a.window, a.sinks, 7);
+            const KeyBlocks kb = key_blocks(max(s.len - 1 - (ROWS - 1) / a.G, 0), s.len - 1, a.window, a.sinks, 7);
             key = n ? kb.count : -1;
             keys[b] = key;
         }
@@ -201,10 +208,10 @@ __device__ __forceinline__ bool find_prompt_item(const PagedAttn& a, int item, i
 }
 
 template <int D, bool S8>
-__global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PromptParams p) {
-    using SM = PromptSmem<D>;
-    using SH = PromptShape<S8>;
-    constexpr int SLOTS = SM::SLOTS, HALF = SM::HALF, PR_MMA = SH::MMA, PR_THREADS = SH::THREADS;
+__global__ void __launch_bounds__(PromptShape<D, S8>::THREADS, PromptShape<D, S8>::CTAS) paged_prompt_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const PromptParams p) {
+    using SM = PromptSmem<D, S8>;
+    using SH = PromptShape<D, S8>;
+    constexpr int SLOTS = SM::SLOTS, HALF = SM::HALF, PR_ROWS = SH::ROWS, PR_LOADER = SH::LOADER, PR_MMA = SH::MMA, PR_THREADS = SH::THREADS;
     // no static shared memory: the dynamic part then begins at a multiple of 1024, as the swizzle wants it
     extern __shared__ __align__(1024) unsigned char smem[];
     int& odd_value = *(int*)(smem + SM::BARS + 368);
@@ -235,12 +242,12 @@ __global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kern
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if (warp == PR_MMA) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_holder)), "r"(512u) : "memory");
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&tmem_holder)), "r"((unsigned)SH::COLUMNS) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
     asm volatile("griddepcontrol.wait;" ::: "memory");
     PromptItem it;
-    const bool has_item = find_prompt_item<PR_THREADS>(a, (int)(blockIdx.x / p.splits), (int)(blockIdx.x % p.splits), p.splits, blockIdx.x == 0, &it, (FindSpace*)(smem + SM::FIND));
+    const bool has_item = find_prompt_item<PR_ROWS, PR_THREADS>(a, (int)(blockIdx.x / p.splits), (int)(blockIdx.x % p.splits), p.splits, blockIdx.x == 0, &it, (FindSpace*)(smem + SM::FIND));
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -295,7 +302,7 @@ __global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kern
         const bool mine = w < tiles && i < it.rows;
         const int packed = it.row0 + i, row = over_group(p, packed), place = first_place + row;
         const unsigned lanes = (unsigned)(warp & 3) << 21;              // lane quarter of tensor memory
-        const unsigned to = tmem + 256 + w * D + lanes;
+        const unsigned to = tmem + SH::O_AT + w * D + lanes;
         const float c = a.scale_log2e;
         float m_used = -INFINITY, l = 0.0f;
         unsigned phase = 0, v_phase = 1;                                // v_phase: of the products with V that have been asked for
@@ -692,7 +699,7 @@ __global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kern
             }
         }
         all_done();
-    } else if (warp < PR_MMA + 2) {
+    } else if (warp < PR_MMA + SH::TILES) {
         // ---- products of tile w ----
         const int w = warp - PR_MMA;
         const unsigned idesc_s = make_idesc_bf16(PR_BLOCK / 2, false), idesc_o = make_idesc_bf16(D, true);
@@ -701,7 +708,7 @@ __global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kern
         bool alive = work && n > 0 && w < tiles, begun = false;
         unsigned p_phase = 0, phase = 0;                     // phase: of the ring, at slot `slot`
         int slot = 0;
-        const unsigned ts = tmem + w * 128, to = tmem + 256 + w * D, bs = bar_s + 8 * w, bp = bar_p + 8 * w, bv = bar_v + 8 * w;
+        const unsigned ts = tmem + w * 128, to = tmem + SH::O_AT + w * D, bs = bar_s + 8 * w, bp = bar_p + 8 * w, bv = bar_v + 8 * w;
         const unsigned long long q_desc = make_smem_desc(smem_u32(smem + w * SM::TILE)), k_desc = make_smem_desc(smem_u32(ring)),
                                  v_desc = make_smem_desc_nmajor(smem_u32(ring), HALF);
         auto wait = [&](unsigned bar, unsigned parity) { alive = alive && __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit)); };
@@ -784,7 +791,7 @@ __global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kern
         if (w != 0) return;
         if (lane == 0 && abort_flag_word) atomicExch(a.c.status, 4);
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"((unsigned)SH::COLUMNS) : "memory");
     } else {
         all_done();
     }
@@ -792,13 +799,14 @@ __global__ void __launch_bounds__(PromptShape<S8>::THREADS, 1) paged_prompt_kern
 
 // Merges the sub-states of tiles whose blocks several CTAs shared: a warp per packed row.
 constexpr int PRC_CTAS = 16;      // CTAs of a tile: 16 rows each
-template <int D>
+template <int D, bool S8>
 __global__ void __launch_bounds__(128) paged_prompt_combine_kernel(const PromptParams p) {
+    constexpr int PR_ROWS = PromptShape<D, S8>::ROWS;
     __shared__ FindSpace space;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const PagedAttn& a = p.a;
     PromptItem it;
-    if (!find_prompt_item<128>(a, (int)(blockIdx.x / PRC_CTAS), 0, p.splits, false, &it, &space) || it.splits < 2) return;
+    if (!find_prompt_item<PR_ROWS, 128>(a, (int)(blockIdx.x / PRC_CTAS), 0, p.splits, false, &it, &space) || it.splits < 2) return;
     const int lane = threadIdx.x & 31;
     constexpr int N = D / 32;
     for (int i = blockIdx.x % PRC_CTAS * 4 + (threadIdx.x >> 5); i < it.rows; i += PRC_CTAS * 4) {
@@ -842,10 +850,12 @@ inline bool make_page_map(CUtensorMap* map, const void* base, int D, const Paged
 
 template <int D, bool S8>
 int launch_paged_prompt(PagedAttn a, float scale, cudaStream_t s) {
-    using SM = PromptSmem<D>;
+    using SM = PromptSmem<D, S8>;
+    using SH = PromptShape<D, S8>;
     static std::atomic<unsigned long long> attr_devices{0};
     const int arc = once_per_device(attr_devices, [] {
         B200FC_CUDA(cudaFuncSetAttribute(paged_prompt_kernel<D, S8>, cudaFuncAttributeMaxDynamicSharedMemorySize, SM::BYTES));
+        B200FC_CUDA(cudaFuncSetAttribute(paged_prompt_kernel<D, S8>, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
         return (int)B200FC_OK;
     });
     if (arc) return arc;
@@ -857,13 +867,13 @@ int launch_paged_prompt(PagedAttn a, float scale, cudaStream_t s) {
     p.a = a;
     p.wait_limit_ns = wait_limit_ns();
     // tiles: full ones, and one more of each sequence
-    const long long bound = ((long long)a.c.T * a.G / PR_ROWS + std::min(a.c.B, a.c.T)) * a.c.Hkv;
-    const long long by_rows = (long long)a.c.B * (((long long)a.c.max_rows * a.G + PR_ROWS - 1) / PR_ROWS) * a.c.Hkv;
+    const long long bound = ((long long)a.c.T * a.G / SH::ROWS + std::min(a.c.B, a.c.T)) * a.c.Hkv;
+    const long long by_rows = (long long)a.c.B * (((long long)a.c.max_rows * a.G + SH::ROWS - 1) / SH::ROWS) * a.c.Hkv;
     const long long items = std::min(bound, by_rows);
     int dev = 0, sms = 148;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    p.splits = (int)std::max(1LL, std::min<long long>(std::min<long long>(16, sms / items), (a.c.capacity / PR_BLOCK + 1) / 2));
+    p.splits = (int)std::max(1LL, std::min<long long>(std::min<long long>(16, sms * SH::CTAS / items), (a.c.capacity / PR_BLOCK + 1) / 2));
     if (items * p.splits > 1 << 25) { set_error("paged_attention: too many rows and heads for one call"); return B200FC_ERR_INVALID; }
     CUtensorMap maps[2] = {};
     p.tma = !S8 && make_page_map(&maps[0], a.c.k, D, a.c) && make_page_map(&maps[1], a.c.v, D, a.c);
@@ -871,7 +881,7 @@ int launch_paged_prompt(PagedAttn a, float scale, cudaStream_t s) {
     bool own = false;
     p.ws_o = p.ws_ml = nullptr;
     if (p.splits > 1) {
-        const size_t states = (size_t)items * p.splits * PR_ROWS;
+        const size_t states = (size_t)items * p.splits * SH::ROWS;
         const int rc = get_stream_scratch(states * (D + 2) * sizeof(float), s, 8, &ws, &own);
         if (rc) return rc;
         p.ws_o = (float*)ws;
@@ -882,7 +892,7 @@ int launch_paged_prompt(PagedAttn a, float scale, cudaStream_t s) {
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)(items * p.splits));
-    cfg.blockDim = dim3(PromptShape<S8>::THREADS);
+    cfg.blockDim = dim3(SH::THREADS);
     cfg.dynamicSmemBytes = SM::BYTES;
     cfg.stream = s;
     cfg.attrs = attr;
@@ -894,7 +904,7 @@ int launch_paged_prompt(PagedAttn a, float scale, cudaStream_t s) {
             cfg.gridDim = dim3((unsigned)(items * PRC_CTAS));
             cfg.blockDim = dim3(128);
             cfg.dynamicSmemBytes = 0;
-            e = cudaLaunchKernelEx(&cfg, paged_prompt_combine_kernel<D>, (const PromptParams)p);
+            e = cudaLaunchKernelEx(&cfg, paged_prompt_combine_kernel<D, S8>, (const PromptParams)p);
             if (e == cudaSuccess) count_launch();
         }
     }
