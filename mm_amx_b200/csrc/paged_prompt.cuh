@@ -5,7 +5,8 @@
 // where the call has too few tiles for the GPU.  Packing the heads of a group into the rows keeps K and V of a block in shared memory for all of them.
 // With heads of 64 in bf16 a CTA takes one tile, and an SM two CTAs: what a CTA does before its first block and after its last (7 us) then runs under the
 // other's blocks, and the last tiles are shorter (6000 rows, window 1000, 16 heads: 94 us with two tiles, 83 with one; 2 x up to 2048 rows, 4096 tokens, 16
-// heads: 78 / 62).  Heads of 128 have no room for that in shared memory, and 8 bits would be widened twice.
+// heads: 78 / 60).  Heads of 128 have room for that only with a ring of
+// 64-token slots (3 sequences of up to 2048 rows: 246 us, and 200 without any loads, where two tiles take 182), and 8 bits would be widened twice.
 //   warps 0-3, 4-7   softmax of tile 0, 1: a thread has one row.  S comes from tensor memory 64 tokens at a time, exp2(S - max) goes back over it as bf16.  The
 //                    maximum that is subtracted follows the true one only when that is 2^8 ahead (sums and values are fp32 and stay far from their limits, the
 //                    probabilities' rounding is relative), so that O in tensor memory is rescaled hardly ever.
@@ -231,7 +232,7 @@ __global__ void __launch_bounds__(PromptShape<D, S8>::THREADS, PromptShape<D, S8
     const unsigned long long limit = p.wait_limit_ns;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < SLOTS; i++) { mbar_init(bar_full + 8 * i, PR_MMA - PR_LOADER); mbar_init(bar_empty + 8 * i, 2); }
+        for (int i = 0; i < SLOTS; i++) { mbar_init(bar_full + 8 * i, PR_MMA - PR_LOADER); mbar_init(bar_empty + 8 * i, SH::TILES); }
         for (int w = 0; w < 2; w++) {
             mbar_init(bar_s + 8 * w, 1); mbar_init(bar_s + 16 + 8 * w, 1);
             mbar_init(bar_p + 8 * w, 4); mbar_init(bar_p + 16 + 8 * w, 4);
@@ -704,7 +705,7 @@ __global__ void __launch_bounds__(PromptShape<D, S8>::THREADS, PromptShape<D, S8
         const int w = warp - PR_MMA;
         const unsigned idesc_s = make_idesc_bf16(PR_BLOCK / 2, false), idesc_o = make_idesc_bf16(D, true);
         auto needed = [&](int j) { return (meta[j % PR_META].facts & 256u << w) != 0; };       // (of a block whose K has arrived)
-        const int frees = tiles == 1 ? 2 : 1;                // arrivals of this tile on a slot's barrier (a lone tile's for both)
+        const int frees = SH::TILES == 2 && tiles == 1 ? 2 : 1;               // arrivals of this tile on a slot's barrier (a lone tile's for both)
         bool alive = work && n > 0 && w < tiles, begun = false;
         unsigned p_phase = 0, phase = 0;                     // phase: of the ring, at slot `slot`
         int slot = 0;
