@@ -313,8 +313,8 @@ __global__ void __launch_bounds__(PromptShape<D, S8>::THREADS, PromptShape<D, S8
         };
         // Heads of 128: the two tiles begin their exponentials in turns (tile 0, tile 1, tile 0, ...); side by side, the unit that computes them would be busy
         // while both need it and idle while both do the rest (3 sequences of up to 2048 rows: 191 us without, 182 with; with turns that are passed on at the end
-        // 189).  One turn for each half of a block, seen or not.  Not where that costs: heads of 64, 6000 rows with a window of 1000, 94 / 100; 8 bits, whose
-        // widening takes as long, no difference.
+        // 189).  One turn for each half of a block, seen or not.  Not for 8 bits, whose
+        // widening takes as long: no difference.
         constexpr bool TURNS = D == 128 && !S8;
         unsigned turn_phase = w == 1 ? 0 : 1;
         auto take_turn = [&] {

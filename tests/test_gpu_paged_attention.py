@@ -49,7 +49,8 @@ def test_few_rows(rows, lens, Hkv, G, D, page, int8, window, sinks):
 
 
 PROMPTS = [([100], [100], 2, 2, 64, 16), ([128, 256, 129], [128, 256, 129], 1, 4, 128, 32), ([257, 1, 0, 65], [600, 400, 5, 65], 2, 3, 128, 64),
-           ([513], [2000], 1, 8, 64, 128), ([300, 40], [280, 0], 2, 1, 128, 16), ([700, 1500], [700, 2047], 1, 2, 128, 64), ([31, 33, 500], [1031, 33, 777], 2, 7, 64, 16)]
+           ([513], [2000], 1, 8, 64, 128), ([300, 40], [280, 0], 2, 1, 128, 16), ([700, 1500], [700, 2047], 1, 2, 128, 64), ([31, 33, 500], [1031, 33, 777], 2, 7, 64, 16),
+           ([127, 128, 129, 1], [127, 400, 129, 900], 2, 1, 64, 32), ([1000, 200], [3000, 200], 1, 3, 64, 128)]
 
 
 @pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
@@ -137,6 +138,18 @@ def test_rows_of_q_that_are_no_numbers(rows, lens):
     got = c.attend()
     capi.sync_check()
     c.check(got, want, mag)
+
+
+@pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rows", [[1, 1], [3, 5], [300, 40]], ids=str)
+def test_kv_heads_that_lie_on_one_another(rows, D, int8):
+    """a head stride of 0 (which no tensor map has)"""
+    c = Paged(rows, [700, 333], 2, 4, D, 32, int8)
+    c.pool = [t[:, :1].expand(-1, 2, -1, -1) for t in c.pool]
+    assert c.cache().head_stride == 0
+    run(c)
+    run(c, window=100, sinks=40)
 
 
 @pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
