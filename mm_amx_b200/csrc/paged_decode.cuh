@@ -64,7 +64,7 @@ __global__ void __launch_bounds__(DEC_THREADS, DecSmem<D, S8, NT>::CTAS) paged_d
     using SM = DecSmem<D, S8, NT>;
     constexpr int CHUNKS = SM::CHUNKS, KSTEPS = D / 16, DEC_STAGES = SM::STAGES;
     extern __shared__ unsigned char dec_smem_raw[];
-    __shared__ int warp_sum[DEC_WARPS], odd_value;
+    __shared__ int warp_sum[DEC_WARPS];
     __shared__ struct { DecSeq seq; int b, hk, j; } first;
     unsigned char* smem = dec_smem_raw + (((smem_u32(dec_smem_raw) + 127u) & ~127u) - smem_u32(dec_smem_raw));
     float* st_o = (float*)(smem + SM::RING);                  // states of two warps
@@ -419,19 +419,18 @@ __global__ void __launch_bounds__(DEC_THREADS, DecSmem<D, S8, NT>::CTAS) paged_d
                 }
             }
         };
-        if (threadIdx.x == 0) odd_value = 0;
         __syncthreads();                                  // (the previous pair's states have been read)
-        if (odd) odd_value = 1;
         put_ml(warp);
         if (warp >= 2) put_state(st_o + (warp - 2) * SM::WARP_STATE);
-        __syncthreads();
+        // (every thread gets the answer from the barrier: a shared word would have to be cleared for the next pair while late warps still read it)
+        const bool any_odd = __syncthreads_or(odd);
         if (warp < 2) take_state(st_o + warp * SM::WARP_STATE, warp + 2);
         __syncwarp();
         if (warp == 1) { put_ml(1); put_state(st_o + SM::WARP_STATE); }
         __syncthreads();
         const bool split = run0 > 0 || run1 < units;
         const size_t sub = ((size_t)blockIdx.x * 2 + (run0 > 0 ? 0 : 1)) * 16;
-        if (odd_value && s.rows > 1) {
+        if (any_odd && s.rows > 1) {
             // a value that is no number stands in a block that some rows do not see: row by row, each over what it sees
             for (int i = warp; i < rows; i += DEC_WARPS)
                 row_state<D, S8>(a, at_b, s, i / a.G, at_hk * a.G + i % a.G, kb, 4, 4 * run0, min(4 * run1, kb.count), split ? p.ws_o + (sub + i) * D : nullptr,

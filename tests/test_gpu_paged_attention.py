@@ -303,3 +303,19 @@ def test_the_same_call_gives_the_same_bits(rows, lens, int8):
     for _ in range(5):
         assert torch.equal(c.attend(), first)
     capi.sync_check()
+
+
+@pytest.mark.parametrize("D,window", [(64, 0), (128, 0), (64, 9)])
+def test_pairs_with_and_without_odd_values_one_after_another(D, window):
+    """single blocks handle several (sequence, kv head) pairs in turn: a NaN in one pair's newest values neither reaches the next pair nor leaves a row out"""
+    n = 500
+    c = Paged([2 + b % 3 for b in range(n)], [20 + b * 7 % 50 for b in range(n)], 4, 2, D, 16)
+    for b in range(0, n, 2):
+        at = c.lens[b] - 1
+        c.pool[1][c.ids[b][at // 16], b // 2 % 4, at % 16, 9] = float("nan")
+    ref = c.attended(window=window)
+    for _ in range(5):
+        c.out.fill_(7.0)
+        got = c.attend(window=window)
+        capi.sync_check()
+        c.check(got, *ref)
