@@ -340,7 +340,7 @@ int b200fc_kv_append(const b200fc_kv_append_t* a, void* stream);
 
 /* out[r, h, :] = sum_j softmax_j(scale * q[r, h, :] . k_j) v_j over the cached tokens j of the row's sequence that are visible to its place p:
  * j <= p, and with window > 0 only the last `window` of them (j > p - window) and the first `sinks` tokens of the sequence (j < sinks).  Rows that see no
- * token are zeros.  Scores, softmax and sums are fp32; probabilities are rounded to bf16 for the product with v.  H / Hkv query heads share a kv head
+ * token, or none whose score is more than -inf, are zeros.  Scores, softmax and sums are fp32; probabilities are rounded to bf16 for the product with v.  H / Hkv query heads share a kv head
  * (any number).  max_rows, at least 1: no sequence has more rows (a sequence that has is left out, as above).  q and out bf16, 16-byte aligned with their strides; out overlaps
  * neither q nor the cache.  scale: any number below 2^127.
  * What lies behind a sequence's last token, or is invisible to all its rows, may be anything, NaN included.  k and v of visible tokens: any bf16. */

@@ -10,6 +10,7 @@
 // probabilities turn from one form into the other by movmatrix.  (tcgen05 would work on 128 rows; bytes bound this: 23 per clock and SM at HBM speed.)
 // 8 bits: bytes become bf16 of (value / 64), exactly, in two instructions a pair; the page's factors go into the scores and into the probabilities.
 #pragma once
+#include <cfloat>
 #include "paged_common.cuh"
 
 namespace b200fc {
@@ -215,7 +216,7 @@ __global__ void __launch_bounds__(DEC_THREADS, DecSmem<D, S8, NT>::CTAS) paged_d
 #pragma unroll
             for (int r = 0; r < 2; r++) {
                 place[nt][r] = s.len - s.rows + (8 * nt + 2 * t + r) / a.G;
-                m_run[nt][r] = -INFINITY;
+                m_run[nt][r] = -FLT_MAX;                          // (not -inf: scores of -inf, masked or not, then weigh 0 without a look at them)
                 l_run[nt][r] = 0.0f;
             }
         }
@@ -302,7 +303,7 @@ __global__ void __launch_bounds__(DEC_THREADS, DecSmem<D, S8, NT>::CTAS) paged_d
                     float f[2];
 #pragma unroll
                     for (int r = 0; r < 2; r++) {
-                        f[r] = top[nt][r] == -INFINITY ? 1.0f : exp2_approx(m_run[nt][r] - top[nt][r]);
+                        f[r] = exp2_approx(m_run[nt][r] - top[nt][r]);
                         m_run[nt][r] = top[nt][r];
                         l_run[nt][r] *= f[r];
                     }
@@ -319,9 +320,9 @@ __global__ void __launch_bounds__(DEC_THREADS, DecSmem<D, S8, NT>::CTAS) paged_d
 #pragma unroll
                 for (int c = 0; c < 4; c++) {
                     const float x = sc[nt][c];
-                    e[c] = whole || x != -INFINITY ? exp2_approx(x - m_run[nt][c & 1]) : 0.0f;
+                    e[c] = exp2_approx(x - m_run[nt][c & 1]);
                     l_run[nt][c & 1] += e[c];
-                    if (S8) e[c] = whole || x != -INFINITY ? e[c] * fv : 0.0f;
+                    if (S8 && (whole || x != -INFINITY)) e[c] *= fv;          // (a masked token has no part in its page's factor, which may be NaN)
                 }
                 // (token g, rows 2 t, 2 t + 1) -> (row g, tokens 2 t, 2 t + 1)
                 pb[nt][0] = transpose8x8(pack2_bf16(e[0], e[1]));
@@ -406,8 +407,8 @@ __global__ void __launch_bounds__(DEC_THREADS, DecSmem<D, S8, NT>::CTAS) paged_d
                 for (int r = 0; r < 2; r++) {
                     const float2 ml = *(const float2*)(st_ml + (w * 16 + 8 * nt + 2 * t + r) * 2);
                     const float m = fmaxf(m_run[nt][r], ml.x);
-                    f[r] = m_run[nt][r] == -INFINITY ? 0.0f : exp2_approx(m_run[nt][r] - m);
-                    e[r] = ml.x == -INFINITY ? 0.0f : exp2_approx(ml.x - m);
+                    f[r] = exp2_approx(m_run[nt][r] - m);
+                    e[r] = exp2_approx(ml.x - m);
                     l_run[nt][r] = l_run[nt][r] * f[r] + ml.y * e[r];
                     m_run[nt][r] = m;
                 }

@@ -319,3 +319,31 @@ def test_pairs_with_and_without_odd_values_one_after_another(D, window):
         got = c.attend(window=window)
         capi.sync_check()
         c.check(got, *ref)
+
+
+@pytest.mark.parametrize("how", ["infinite", "overflow", "int8"])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("rows,lens,window,sinks", [([1, 1], [400, 150], 0, 0), ([1, 1, 1], [5000, 3, 700], 0, 0), ([1, 1], [3000, 150], 100, 40), ([3, 2], [300, 77], 0, 0),
+                                                    ([8, 5], [3000, 500], 90, 20), ([200, 20], [330, 70], 0, 0), ([300, 40], [900, 300], 100, 30), ([40], [6000], 0, 0)])
+def test_scores_of_minus_infinity(rows, lens, window, sinks, D, how):
+    """visible keys whose score is -inf (an infinity in k, or products beyond fp32) weigh nothing, wherever they stand: all in front of the rows' own places, and every third
+    block of 16 tokens from there on.  (Each row sees a token with another score: its sequence's first row's, or one of the two blocks between.)"""
+    c = Paged(rows, lens, 2, 4, D, 16, how == "int8")
+    big = 2.0 ** 127
+    c.q[..., 3] = 1.0 if how == "infinite" else big
+    for b, n in enumerate(lens):
+        for j in range(n):
+            low = j < n - rows[b] or j // 16 % 3 == 0 and j > n - rows[b]
+            c.pool[0][c.ids[b][j // 16], :, j % 16, 3] = 0 if not low else {"infinite": float("-inf"), "overflow": -big, "int8": -127}[how]
+    run(c, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("rows,lens", [([1, 1], [400, 3]), ([4, 2], [300, 7]), ([200, 20], [330, 70]), ([40], [6000])])
+def test_rows_whose_every_score_is_minus_infinity(rows, lens):
+    c = Paged(rows, lens, 2, 4, 128, 16)
+    c.q[..., 3] = 1.0
+    for b, n in enumerate(lens):
+        c.pool[0][c.ids[b], :, :, 3] = float("-inf")
+    got = c.attend()
+    capi.sync_check()
+    assert bool((got == 0).all())
