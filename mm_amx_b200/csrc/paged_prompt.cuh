@@ -179,7 +179,7 @@ __device__ __forceinline__ bool find_prompt_item(const PagedAttn& a, int item, i
         __syncthreads();
     } else {
         long long seen = 0;
-        for (int b0 = 0; b0 < a.c.B && seen <= item; b0 += THREADS) {
+        for (int b0 = 0; b0 < a.c.B && (seen <= item || report); b0 += THREADS) {      // (who reports looks at all of them)
             const int b = b0 + threadIdx.x;
             SeqRows s;
             int tiles = 0;

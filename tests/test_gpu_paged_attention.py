@@ -347,3 +347,36 @@ def test_rows_whose_every_score_is_minus_infinity(rows, lens):
     got = c.attend()
     capi.sync_check()
     assert bool((got == 0).all())
+
+
+@pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("n,rows", [(700, 5), (20, 9), (300, 1)])
+def test_every_sequence_outside_its_buffers_is_reported(n, rows, int8):
+    """wherever it stands among the call's sequences, with rows or without; the others get their results"""
+    rows = [0 if b % 9 == 7 else rows for b in range(n)]
+    c = Paged(rows, [9 + b % 7 for b in range(n)], 1, 8, 64, 16, int8)
+    ref, mag = c.attended()
+    starts, lens = c.row_start.clone(), c.seq_lens.clone()
+
+    def broken(harmed):
+        c.out.fill_(7.0)
+        c.attend()
+        with pytest.raises(capi.B200FCError) as e:
+            capi.sync_check()
+        assert e.value.code == capi.ERR_INVALID
+        over = (c.out[:, :c.H].double() - ref).abs() - (2.0 ** -8 * 1.01 * (mag + ref.abs()) + 3e-4 * mag)
+        unharmed = torch.ones(c.T, dtype=torch.bool, device="cuda")
+        for b in harmed:
+            unharmed[c.starts[b]:c.starts[b + 1]] = False
+            assert bool((c.out[c.starts[b]:c.starts[b + 1]] == 7.0).all())
+        assert float(over[unharmed].max()) <= 0
+        c.row_start.copy_(starts); c.seq_lens.copy_(lens)
+
+    for b in {0, 7, n // 3, n // 2 + 1, 63 % n, 64 % n, 256 % n, 691 % n, n - 1}:
+        for length in (-1, 2 ** 31 - 1, c.table.shape[1] * 16 + 1):
+            c.seq_lens[b] = length
+            broken([b])
+    c.row_start[n] = c.T + 1
+    broken([n - 1])
+    c.row_start[n - 5] = -1
+    broken([n - 6, n - 5])
