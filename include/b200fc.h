@@ -292,7 +292,7 @@ int b200fc_decode_attention(const b200fc_attention_t* a, void* stream);
  * int8 * factor.
  * D: 64 or 128.  page_tokens: 16, 32, 64 or 128.  k, v and their strides 16-byte aligned, token_stride >= a token's D elements.
  * Everything that page_table, seq_lens and row_start name is checked where it is read, on the device.  A sequence whose rows or length lie outside
- * their buffers is left out (its rows of out are not written), a page outside [0, pages) is neither written nor read, and the next
+ * their buffers is left out (its rows of out are not written; where row_start falls, rows of others may be left out of the append too), a page outside [0, pages) is neither written nor read, and the next
  * b200fc_sync_check on the device returns B200FC_ERR_INVALID once.  Table entries behind a sequence's last token may hold anything. */
 typedef struct {
     int pages, page_tokens, Hkv, D, dtype;

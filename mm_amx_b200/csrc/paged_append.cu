@@ -28,7 +28,7 @@ struct AppendParams {
     const int* positions; long long position_stride;            // entries
     int axes, sec0, sec01;                             // pairs below sec0 take axis 0, below sec01 axis 1
     int row_groups;                                    // CTAs that share a row
-    int page_ctas;                                     // 8-bit cache: CTAs [0, page_ctas) take pages, the others rows of q
+    int check_ctas, page_ctas;                         // the first CTAs look the sequences over, the next (8-bit cache) take pages, the others rows
 };
 
 __device__ __forceinline__ float bf_lo(unsigned w) { return __uint_as_float(w << 16); }
@@ -130,10 +130,7 @@ __device__ __forceinline__ void append_row(const AppendParams& p, int r, int gro
     const int b = find_sequence(p.c, r);
     if (b < 0) return;
     SeqRows s;
-    if (!load_seq(p.c, b, &s)) {
-        if (threadIdx.x == 0) report_paged(p.c);
-        return;
-    }
+    load_seq(p.c, b, &s);
     if (r < s.row0 || r >= s.row0 + s.rows) return;
     const int place = s.len - s.rows + (r - s.row0);
     if (place < 0) return;
@@ -184,7 +181,7 @@ __device__ __forceinline__ void append_page(const AppendParams& p, int segment, 
     int b = -1, index = 0;
     for (int b0 = 0; b0 < p.c.B; b0 += 32) {
         SeqRows mine{0, 0, 0};
-        if (b0 + lane < p.c.B && !load_seq(p.c, b0 + lane, &mine) && segment == 0 && threadIdx.x < 32) report_paged(p.c);
+        if (b0 + lane < p.c.B) load_seq(p.c, b0 + lane, &mine);
         const int n = touched_pages(mine, shift);
         int upto = n;
 #pragma unroll
@@ -313,7 +310,13 @@ __device__ __forceinline__ void append_page(const AppendParams& p, int segment, 
 
 template <int D, bool S8>
 __global__ void __launch_bounds__(APP_THREADS) kv_append_kernel(const AppendParams p) {
-    const int cta = blockIdx.x;
+    const int cta = (int)blockIdx.x - p.check_ctas;
+    if (cta < 0) {                                     // reports sequences whose numbers lie outside their buffers, whether they have rows or not
+        const int b = blockIdx.x * APP_THREADS + threadIdx.x;
+        SeqRows s;
+        if (b < p.c.B && !load_seq(p.c, b, &s)) report_paged(p.c);
+        return;
+    }
     if (S8 && cta < p.page_ctas) {
         const int part = cta % (2 * p.c.Hkv);
         append_page<D>(p, cta / (2 * p.c.Hkv), part >> 1, part & 1);
@@ -376,9 +379,10 @@ int launch_kv_append(const b200fc_kv_append_t& a, cudaStream_t s) {
     const long long page_ctas = s8 ? segments * 2 * c.Hkv : 0;
     p.row_groups = 1;
     const long long row_ctas = s8 && !p.H ? 0 : (long long)a.T * p.row_groups;
-    if (page_ctas + row_ctas > 0x7fffffffLL) { set_error("kv_append: too many rows and heads for one call"); return B200FC_ERR_INVALID; }
-    p.page_ctas = (int)page_ctas;
-    const dim3 grid((unsigned)(page_ctas + row_ctas));
+    const long long check_ctas = (c.B + APP_THREADS - 1) / APP_THREADS;
+    if (page_ctas + row_ctas + check_ctas > 0x7fffffffLL) { set_error("kv_append: too many rows and heads for one call"); return B200FC_ERR_INVALID; }
+    p.check_ctas = (int)check_ctas; p.page_ctas = (int)page_ctas;
+    const dim3 grid((unsigned)(page_ctas + row_ctas + check_ctas));
     if (c.D == 128) s8 ? kv_append_kernel<128, true><<<grid, APP_THREADS, 0, s>>>(p) : kv_append_kernel<128, false><<<grid, APP_THREADS, 0, s>>>(p);
     else s8 ? kv_append_kernel<64, true><<<grid, APP_THREADS, 0, s>>>(p) : kv_append_kernel<64, false><<<grid, APP_THREADS, 0, s>>>(p);
     B200FC_CUDA(cudaGetLastError());

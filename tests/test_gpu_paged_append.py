@@ -229,6 +229,39 @@ def test_what_is_out_of_range_is_reported_and_left_out(int8):
     capi.sync_check()
 
 
+@pytest.mark.parametrize("with_q", [True, False])
+@pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("rows", [[0 if b % 5 == 2 else 3 for b in range(300)], [1] * 32 + [0] * 40, [0, 0, 2]], ids=["many", "none behind", "few"])
+def test_every_sequence_outside_its_buffers_is_reported(rows, int8, with_q):
+    """wherever it stands among the call's sequences, with rows or without; the others' pages are filled as without it"""
+    n = len(rows)
+    c, want = (Paged(rows, [9 + b % 7 for b in range(n)], 1, 2, 64, 16, int8) for _ in range(2))
+    append(want, with_q=with_q)
+    capi.sync_check()
+    starts, lens = c.row_start.clone(), c.seq_lens.clone()
+
+    def broken(harmed):
+        append(c, with_q=with_q)
+        with pytest.raises(capi.B200FCError) as e:
+            capi.sync_check()
+        assert e.value.code == capi.ERR_INVALID
+        c.row_start.copy_(starts); c.seq_lens.copy_(lens)
+        fine = [pg for b in range(n) if b not in harmed for pg in c.ids[b]]
+        for i in range(2):
+            assert torch.equal(c.pool[i][fine].view(torch.int8), want.pool[i][fine].view(torch.int8))
+
+    for b in sorted({0, 2 % n, 33 % n, 137 % n, n - 3, n - 1}):
+        for length in (-1, 2 ** 31 - 1, c.table.shape[1] * 16 + 1):
+            c.seq_lens[b] = length
+            broken([b])
+    c.row_start[n] = c.T + 1
+    broken([n - 1])
+    c.row_start[n - 1] = -1
+    broken(range(n))                     # (where row_start falls, rows of other sequences may not be found)
+    c.row_start[n - 1] = c.T + 1
+    broken([n - 2, n - 1])
+
+
 def test_captured_and_replayed():
     """lengths and pages move on between replays"""
     for int8 in (False, True):
