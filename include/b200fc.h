@@ -343,7 +343,9 @@ int b200fc_kv_append(const b200fc_kv_append_t* a, void* stream);
  * token, or none whose score is more than -inf, are zeros.  Scores, softmax and sums are fp32; probabilities are rounded to bf16 for the product with v.  H / Hkv query heads share a kv head
  * (any number).  max_rows, at least 1: no sequence has more rows (a sequence that has is left out, as above).  q and out bf16, 16-byte aligned with their strides; out overlaps
  * neither q nor the cache.  scale: any number below 2^127.
- * What lies behind a sequence's last token, or is invisible to all its rows, may be anything, NaN included.  k and v of visible tokens: any bf16. */
+ * What lies behind a sequence's last token, or is invisible to all its rows, may be anything, NaN included.  k and v of visible tokens: any bf16, infinities
+ * and NaN too; but the weights of v are divided by their sum only at the end, and may be 2^8 until then, so the result is finite only while the largest
+ * finite |v| times the row's visible tokens is below 2^119.  8-bit cache: so too with |v| = 127 * v_scale, and k_scale and k_scale * |scale| below 2^121. */
 typedef struct {
     const b200fc_paged_cache_t* cache;
     int T, max_rows, H;

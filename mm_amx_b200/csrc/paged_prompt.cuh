@@ -8,8 +8,9 @@
 // heads: 78 / 60).  Heads of 128 have room for that only with a ring of
 // 64-token slots (3 sequences of up to 2048 rows: 246 us, and 200 without any loads, where two tiles take 182), and 8 bits would be widened twice.
 //   warps 0-3, 4-7   softmax of tile 0, 1: a thread has one row.  S comes from tensor memory 64 tokens at a time, exp2(S - max) goes back over it as bf16.  The
-//                    maximum that is subtracted follows the true one only when that is 2^8 ahead (sums and values are fp32 and stay far from their limits, the
-//                    probabilities' rounding is relative), so that O in tensor memory is rescaled hardly ever.
+//                    maximum that is subtracted follows the true one only when that is 2^8 ahead, so that O in tensor memory is rescaled hardly ever (the
+//                    probabilities' rounding is relative; sums of p v are fp32 and reach 2^8 * tokens * |v|, which bounds v.  A smaller scale would end that
+//                    bound, but lose probabilities near 2^-126, which sharply peaked rows with zeros in v at their peak show).
 //   2, 4 or 8 more   fetch K and V blocks into a ring of 128-token slots (128-byte swizzle): bf16 by TMA, or in blocks that not every row sees by cp.async with zeros
 //                    for tokens that nobody sees (which may hold anything), 8 bits widened on the way to bf16 of (value / 64), exactly; the page's factors go to the softmax.
 //   one a tile       issues its products: S_w = Q_w K^T (Q, K in shared memory), O_w += P_w V (P in tensor memory, V as it lies: N-major).  One

@@ -1,4 +1,6 @@
 """GPU: attention over the paged cache (b200fc_paged_attention) against the formula in 64 bits."""
+import math
+
 import pytest
 import torch
 
@@ -380,3 +382,41 @@ def test_every_sequence_outside_its_buffers_is_reported(n, rows, int8):
     broken([n - 1])
     c.row_start[n - 5] = -1
     broken([n - 6, n - 5])
+
+
+@pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
+@pytest.mark.parametrize("rows,lens", [([1, 1, 1], [9000, 3, 700]), ([3, 2], [3000, 77]), ([200, 140], [330, 700]), ([40], [20000])])
+@pytest.mark.parametrize("D", [64, 128])
+def test_the_largest_values(D, rows, lens, int8):
+    """|v| times the visible tokens just below 2^119, with scores behind the first 128 tokens that are 7.9 / log2(e) higher, so that weights reach nearly 2^8.  (The sums
+    of p v are then below 2^127 (1 + 2^-7): finite.)"""
+    c = Paged(rows, lens, 2, 4, D, 16, int8, std=0.02)
+    c.q[..., 3] = 8.0
+    size = 0.99 * 2.0 ** 119 / max(lens)
+    sign = torch.where(torch.rand(2, 1, D, generator=c.g, device="cuda") < 0.5, -1.0, 1.0)
+    for ids in c.ids:
+        for j, pg in enumerate(ids):
+            if int8:
+                c.pool[1][pg] = (127 * sign).to(torch.int8)
+                c.scales[0][pg, :2], c.scales[1][pg, :2] = 0.7 / 127, size / 127
+                c.pool[0][pg, ..., 3] = 0 if j < 8 else 124
+                c.pool[0][pg, ..., :3] = 0
+                c.pool[0][pg, ..., 4:] = 0
+            else:
+                c.pool[1][pg] = (size * sign).to(torch.bfloat16)
+                c.pool[0][pg, ..., 3] = 0.0 if j < 8 else 7.9 / 8 * math.log(2)
+    run(c, scale=1.0)
+    run(c, scale=1.0, window=100, sinks=4)
+
+
+@pytest.mark.parametrize("rows,lens", [([1, 1], [400, 150]), ([3, 2], [300, 77]), ([200, 20], [330, 70])])
+def test_the_largest_factors_of_keys(rows, lens):
+    """k_scale and k_scale * scale just below 2^121, met by rows of q so small that the scores are ordinary (four components of +- 2^-121 against integers of 0 and +- 32:
+    sums of up to four times 32, so that all products and scores are normal numbers of fp32), every other row all zeros"""
+    c = Paged(rows, lens, 2, 4, 64, 16, True)
+    c.scales[0][:, :2].mul_(0.99 * 2.0 ** 121 / float(c.scales[0][c.ids[0] + c.ids[1], :2].max()))
+    c.pool[0].copy_((c.pool[0].float() / 64).round().clamp(-1, 1) * 32)
+    c.q.copy_(torch.sign(c.q) * 2.0 ** -121 * (torch.arange(64, device="cuda") % 16 == 5))
+    c.q[1::2] = 0.0
+    run(c)
+    run(c, scale=1.0)
