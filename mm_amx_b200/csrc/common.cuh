@@ -351,6 +351,10 @@ __device__ __forceinline__ int f32_to_s8(float v) {
 __device__ __forceinline__ unsigned short f32_to_bf16_bits(float v) {
     return __bfloat16_as_ushort(__float2bfloat16_rn(v));
 }
+__device__ __forceinline__ unsigned pack_bf16x2(float lo, float hi) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *(const unsigned*)&h;
+}
 
 // DEQUANT -> BIAS -> GELU -> QUANT on one fp32 value of output column n.
 __device__ __forceinline__ float postop_scalar(float v, int n, const Epilogue& ep) {

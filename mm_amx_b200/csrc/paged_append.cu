@@ -27,7 +27,6 @@ struct AppendParams {
     const float* cos; const float* sin; long long rot_stride;   // floats
     const int* positions; long long position_stride;            // entries
     int axes, sec0, sec01;                             // pairs below sec0 take axis 0, below sec01 axis 1
-    int row_groups;                                    // CTAs that share a row
     int check_ctas, page_ctas;                         // the first CTAs look the sequences over, the next (8-bit cache) take pages, the others rows
 };
 
@@ -93,22 +92,18 @@ __device__ __forceinline__ void turn(const uint4 lo, const uint4 hi, bool turned
         }
     }
 }
-__device__ __forceinline__ unsigned pack2_bf16(float lo, float hi) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *(const unsigned*)&h;
-}
 __device__ __forceinline__ void store_bf16(unsigned char* dst, const Item& it, const float (&y)[16]) {
-    *(uint4*)(dst + 2 * it.lo) = make_uint4(pack2_bf16(y[0], y[1]), pack2_bf16(y[2], y[3]), pack2_bf16(y[4], y[5]), pack2_bf16(y[6], y[7]));
-    *(uint4*)(dst + 2 * it.hi) = make_uint4(pack2_bf16(y[8], y[9]), pack2_bf16(y[10], y[11]), pack2_bf16(y[12], y[13]), pack2_bf16(y[14], y[15]));
+    *(uint4*)(dst + 2 * it.lo) = make_uint4(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]), pack_bf16x2(y[4], y[5]), pack_bf16x2(y[6], y[7]));
+    *(uint4*)(dst + 2 * it.hi) = make_uint4(pack_bf16x2(y[8], y[9]), pack_bf16x2(y[10], y[11]), pack_bf16x2(y[12], y[13]), pack_bf16x2(y[14], y[15]));
 }
 
-// Heads of one row, `groups` CTAs side by side: q, and with a bf16 cache k and v.
+// Heads of one row: q, and with a bf16 cache k and v.
 template <int D, bool S8>
-__device__ __forceinline__ void append_row(const AppendParams& p, int r, int group, int groups) {
+__device__ __forceinline__ void append_row(const AppendParams& p, int r) {
     constexpr int ITEMS = D / 16, SLOTS = APP_THREADS / ITEMS;
     const int i = threadIdx.x % ITEMS, slot = threadIdx.x / ITEMS;
     const Item it = item_of(p, i);
-    const int heads = p.H + (S8 ? 0 : 2 * p.c.Hkv), stride = groups * SLOTS;
+    const int heads = p.H + (S8 ? 0 : 2 * p.c.Hkv);
     auto source = [&](int h) {
         if (h < p.H) return p.q + (long long)r * p.q_rs + (long long)h * p.q_hs;
         const int hk = h - p.H;
@@ -119,13 +114,13 @@ __device__ __forceinline__ void append_row(const AppendParams& p, int r, int gro
     auto load = [&](int h) {
 #pragma unroll
         for (int u = 0; u < 2; u++)
-            if (h + u * stride < heads) {
-                const unsigned char* src = source(h + u * stride);
+            if (h + u * SLOTS < heads) {
+                const unsigned char* src = source(h + u * SLOTS);
                 x[u][0] = *(const uint4*)(src + 2 * it.lo);
                 x[u][1] = *(const uint4*)(src + 2 * it.hi);
             }
     };
-    int h = group * SLOTS + slot;
+    int h = slot;
     load(h);
     const int b = find_sequence(p.c, r);
     if (b < 0) return;
@@ -140,10 +135,10 @@ __device__ __forceinline__ void append_row(const AppendParams& p, int r, int gro
     if (it.turned) ok = load_turn(p, i, r, place, cs, sn) && ok;
     if (!ok) report_paged(p.c);
     const long long token = (long long)(place & ((1 << p.c.page_shift) - 1)) * p.c.token_stride + (long long)page * p.c.page_stride;
-    for (; h < heads; h += 2 * stride, load(h))
+    for (; h < heads; h += 2 * SLOTS, load(h))
 #pragma unroll
         for (int u = 0; u < 2; u++) {
-            const int hh = h + u * stride;
+            const int hh = h + u * SLOTS;
             if (hh >= heads) break;
             unsigned char* dst;
             bool turned = it.turned;
@@ -308,8 +303,10 @@ __device__ __forceinline__ void append_page(const AppendParams& p, int segment, 
     }
 }
 
+// CTAs per SM: 8 bits have as many CTAs as pages, kv heads and k and v, so that those of a step over some 30 sequences are resident together (one row each of 32
+// sequences, 8 kv heads: with 4 per SM 5.2 us, 3 per SM 6.3, 5 per SM 4.8, although 88 bytes are spilled); rows have 74 registers.
 template <int D, bool S8>
-__global__ void __launch_bounds__(APP_THREADS) kv_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(APP_THREADS, S8 ? 5 : 6) kv_append_kernel(const AppendParams p) {
     const int cta = (int)blockIdx.x - p.check_ctas;
     if (cta < 0) {                                     // reports sequences whose numbers lie outside their buffers, whether they have rows or not
         const int b = blockIdx.x * APP_THREADS + threadIdx.x;
@@ -322,8 +319,7 @@ __global__ void __launch_bounds__(APP_THREADS) kv_append_kernel(const AppendPara
         append_page<D>(p, cta / (2 * p.c.Hkv), part >> 1, part & 1);
         return;
     }
-    const int at = cta - p.page_ctas;
-    append_row<D, S8>(p, at / p.row_groups, at % p.row_groups, p.row_groups);
+    append_row<D, S8>(p, cta - p.page_ctas);
 }
 
 }  // namespace
@@ -377,8 +373,7 @@ int launch_kv_append(const b200fc_kv_append_t& a, cudaStream_t s) {
     // pages that the call can touch: (rows - 1) / page_tokens + 2 of each sequence, and no more than rows
     const long long segments = std::min<long long>(a.T, a.T / c.page_tokens + 2LL * c.B);
     const long long page_ctas = s8 ? segments * 2 * c.Hkv : 0;
-    p.row_groups = 1;
-    const long long row_ctas = s8 && !p.H ? 0 : (long long)a.T * p.row_groups;
+    const long long row_ctas = s8 && !p.H ? 0 : (long long)a.T;
     const long long check_ctas = (c.B + APP_THREADS - 1) / APP_THREADS;
     if (page_ctas + row_ctas + check_ctas > 0x7fffffffLL) { set_error("kv_append: too many rows and heads for one call"); return B200FC_ERR_INVALID; }
     p.check_ctas = (int)check_ctas; p.page_ctas = (int)page_ctas;

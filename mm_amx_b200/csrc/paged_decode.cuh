@@ -325,8 +325,8 @@ __global__ void __launch_bounds__(DEC_THREADS, DecSmem<D, S8, NT>::CTAS) paged_d
                     if (S8 && (whole || x != -INFINITY)) e[c] *= fv;          // (a masked token has no part in its page's factor, which may be NaN)
                 }
                 // (token g, rows 2 t, 2 t + 1) -> (row g, tokens 2 t, 2 t + 1)
-                pb[nt][0] = transpose8x8(pack2_bf16(e[0], e[1]));
-                pb[nt][1] = transpose8x8(pack2_bf16(e[2], e[3]));
+                pb[nt][0] = transpose8x8(pack_bf16x2(e[0], e[1]));
+                pb[nt][1] = transpose8x8(pack_bf16x2(e[2], e[3]));
             }
             // ---- O^T += V^T P^T: 16 components x 8 rows ----
             if constexpr (!S8) {
@@ -461,7 +461,7 @@ __global__ void __launch_bounds__(DEC_THREADS, DecSmem<D, S8, NT>::CTAS) paged_d
                     if (split) *(float2*)(p.ws_o + (sub + i) * D + d) = x;
                     else {
                         const float inv = ml.y != 0.0f ? 1.0f / ml.y : 0.0f;
-                        *(unsigned*)(a.out + (long long)(s.row0 + row) * a.o_rs + (long long)(at_hk * a.G + i - row * a.G) * a.o_hs + 2 * d) = pack2_bf16(x.x * inv, x.y * inv);
+                        *(unsigned*)(a.out + (long long)(s.row0 + row) * a.o_rs + (long long)(at_hk * a.G + i - row * a.G) * a.o_hs + 2 * d) = pack_bf16x2(x.x * inv, x.y * inv);
                     }
                 }
                 if (split && lane == 0) *(float2*)(p.ws_ml + (sub + i) * 2) = ml;
@@ -532,7 +532,7 @@ __global__ void __launch_bounds__(128) paged_combine_kernel(const DecParams p) {
     unsigned char* out = a.out + (long long)(s.row0 + row) * a.o_rs + (long long)(hk * a.G + i - row * a.G) * a.o_hs;
     const float inv = l != 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
-    for (int e = 0; e < N; e += 2) *(unsigned*)(out + 2 * (lane * N + e)) = pack2_bf16(acc[e] * inv, acc[e + 1] * inv);
+    for (int e = 0; e < N; e += 2) *(unsigned*)(out + 2 * (lane * N + e)) = pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
 }
 
 template <int D, bool S8, int NT>

@@ -46,7 +46,7 @@ template <int D, bool S8> struct PromptSmem {
     static constexpr int HALF = PR_BLOCK * 128;                       // 128 rows of 64 components
     static constexpr int TILE = HALF * (D / 64);                      // a tile of Q, a block of K or V
     static constexpr int SLOTS = D == 128 || TILES == 1 ? 5 : 8;
-    static constexpr int AHEAD = SLOTS == 5 ? 2 : 3;                     // fetched blocks whose arrival is waited for later
+    static constexpr int AHEAD = 2;                                   // fills by cp.async whose arrival is waited for later
     static constexpr int RING = TILES * TILE, BARS = RING + SLOTS * TILE;
     static constexpr int META = BARS + 384;
     static constexpr int FIND = META + PR_META * 80;                  // for the search for the tile
@@ -800,7 +800,7 @@ __global__ void __launch_bounds__(PromptShape<D, S8>::THREADS, PromptShape<D, S8
 }
 
 // Merges the sub-states of tiles whose blocks several CTAs shared: a warp per packed row.
-constexpr int PRC_CTAS = 16;      // CTAs of a tile: 16 rows each
+constexpr int PRC_CTAS = 16;      // CTAs of a tile: 16 rows each, 8 where a tile has 128
 template <int D, bool S8>
 __global__ void __launch_bounds__(128) paged_prompt_combine_kernel(const PromptParams p) {
     constexpr int PR_ROWS = PromptShape<D, S8>::ROWS;
@@ -832,7 +832,7 @@ __global__ void __launch_bounds__(128) paged_prompt_combine_kernel(const PromptP
         unsigned char* out = a.out + (long long)(it.s.row0 + row) * a.o_rs + (long long)(it.hk * a.G + packed - row * a.G) * a.o_hs;
         const float inv = l != 0.0f ? 1.0f / l : 0.0f;
 #pragma unroll
-        for (int e = 0; e < N; e += 2) *(unsigned*)(out + 2 * (lane * N + e)) = pack2_bf16(acc[e] * inv, acc[e + 1] * inv);
+        for (int e = 0; e < N; e += 2) *(unsigned*)(out + 2 * (lane * N + e)) = pack_bf16x2(acc[e] * inv, acc[e + 1] * inv);
     }
 }
 

@@ -290,10 +290,6 @@ __device__ __forceinline__ void load_col_vec(const float* staged, const float* _
 #pragma unroll
     for (int h = 0; h < 2; h++) { out[2 * h] = pack2(t[h].x, t[h].y); out[2 * h + 1] = pack2(t[h].z, t[h].w); }
 }
-__device__ __forceinline__ unsigned pack_bf16x2(float lo, float hi) {
-    const __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
-    return *(const unsigned*)&h;
-}
 // Post-ops and store of 32 consecutive columns [n, n + 32) of one output row per lane, whose accumulators are in `acc`.  Called by
 // all lanes of the warp.  This is the form for everything: chunks at the ragged end, unaligned outputs, residuals, multicast.
 template <bool HALF = false>
