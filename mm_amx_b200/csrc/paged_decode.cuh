@@ -423,8 +423,11 @@ __global__ void __launch_bounds__(DEC_THREADS, DecSmem<D, S8, NT>::CTAS) paged_d
         __syncthreads();                                  // (the previous pair's states have been read)
         put_ml(warp);
         if (warp >= 2) put_state(st_o + (warp - 2) * SM::WARP_STATE);
-        // (every thread gets the answer from the barrier: a shared word would have to be cleared for the next pair while late warps still read it)
-        const bool any_odd = __syncthreads_or(odd);
+        // has any warp met a value that is no number?  (Every thread gets the answer from the barrier: a shared word would have to be cleared for the next pair while
+        // late warps still read it.)
+        bool any_odd = false;                             // (8 bits hold none)
+        if constexpr (S8) __syncthreads();
+        else any_odd = __syncthreads_or(odd);
         if (warp < 2) take_state(st_o + warp * SM::WARP_STATE, warp + 2);
         __syncwarp();
         if (warp == 1) { put_ml(1); put_state(st_o + SM::WARP_STATE); }

@@ -420,3 +420,19 @@ def test_the_largest_factors_of_keys(rows, lens):
     c.q[1::2] = 0.0
     run(c)
     run(c, scale=1.0)
+
+
+@pytest.mark.parametrize("int8", [False, True], ids=["bf16", "int8"])
+def test_prompts_and_single_tokens_in_two_calls(int8):
+    """the sequences of a mixed batch with prompts first: one call for them, one without row_start for the others, on parts of the same buffers"""
+    c = Paged([150, 40, 1, 1, 1], [400, 40, 900, 1, 77], 2, 4, 128, 32, int8)
+    ref = c.attended()
+    for first, count, row, rows, one_row in ((0, 2, 0, 190, False), (2, 3, 190, 3, True)):
+        cache = c.cache(B=count, page_table=c.table[first:].data_ptr(), seq_lens=c.seq_lens[first:].data_ptr())
+        q, out = c.q[row:], c.out[row:]
+        capi.paged_attention(capi.PagedAttention(
+            cache=capi.pointer(cache), T=rows, max_rows=1 if one_row else 150, H=c.H, row_start=None if one_row else c.row_start.data_ptr(), q=q.data_ptr(),
+            q_row_stride=q.stride(0) * 2, q_head_stride=q.stride(1) * 2, out=out.data_ptr(), out_row_stride=out.stride(0) * 2, out_head_stride=out.stride(1) * 2,
+            scale=c.D ** -0.5))
+    capi.sync_check()
+    c.check(c.out[:, :c.H], *ref)
