@@ -6,7 +6,8 @@
 // With heads of 64 in bf16 a CTA takes one tile, and an SM two CTAs: what a CTA does before its first block and after its last (7 us) then runs under the
 // other's blocks, and the last tiles are shorter (6000 rows, window 1000, 16 heads: 94 us with two tiles, 83 with one; 2 x up to 2048 rows, 4096 tokens, 16
 // heads: 78 / 60).  Heads of 128 have room for that only with a ring of
-// 64-token slots (3 sequences of up to 2048 rows: 246 us, and 200 without any loads, where two tiles take 182), and 8 bits would be widened twice.
+// 64-token slots (3 sequences of up to 2048 rows: 246 us, and 200 without any loads, where two tiles then took 182).  With 8 bits every CTA widens its blocks itself, so two
+// CTAs would widen each block twice; that form was not built.
 //   warps 0-3, 4-7   softmax of tile 0, 1: a thread has one row.  S comes from tensor memory 64 tokens at a time, exp2(S - max) goes back over it as bf16.  The
 //                    maximum that is subtracted follows the true one only when that is 2^8 ahead, so that O in tensor memory is rescaled hardly ever (the
 //                    probabilities' rounding is relative; sums of p v are fp32 and reach 2^8 * tokens * |v|, which bounds v.  A smaller scale would end that
@@ -313,8 +314,8 @@ __global__ void __launch_bounds__(PromptShape<D, S8>::THREADS, PromptShape<D, S8
             if (!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) alive = __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, limit));
         };
         // Heads of 128: the two tiles begin their exponentials in turns (tile 0, tile 1, tile 0, ...); side by side, the unit that computes them would be busy
-        // while both need it and idle while both do the rest (3 sequences of up to 2048 rows: 191 us without, 182 with; with turns that are passed on at the end
-        // 189).  One turn for each half of a block, seen or not.  Not for 8 bits, whose
+        // while both need it and idle while both do the rest (3 sequences of up to 2048 rows: 194.4 us without, 185.4 with, medians of runs in turn; 512 rows over 30000 tokens
+        // 309 / 290; with turns that are passed on at the end a quarter of that is left).  One turn for each half of a block, seen or not.  Not for 8 bits, whose
         // widening takes as long: no difference.
         constexpr bool TURNS = D == 128 && !S8;
         unsigned turn_phase = w == 1 ? 0 : 1;
