@@ -292,8 +292,9 @@ int b200fc_decode_attention(const b200fc_attention_t* a, void* stream);
  * int8 * factor.
  * D: 64 or 128.  page_tokens: 16, 32, 64 or 128.  k, v and their strides 16-byte aligned, token_stride >= a token's D elements.
  * Everything that page_table, seq_lens and row_start name is checked where it is read, on the device.  A sequence whose rows or length lie outside
- * their buffers is left out (its rows of out are not written; where row_start falls, rows of others may be left out of the append too), a page outside [0, pages) is neither written nor read, and the next
- * b200fc_sync_check on the device returns B200FC_ERR_INVALID once.  Table entries behind a sequence's last token may hold anything. */
+ * their buffers is left out (its rows of out are not written; where row_start falls, the append may leave out rows of others too), a page outside
+ * [0, pages) is neither written nor read, and the next b200fc_sync_check on the device returns B200FC_ERR_INVALID once.  Table entries behind a
+ * sequence's last token may hold anything. */
 typedef struct {
     int pages, page_tokens, Hkv, D, dtype;
     void* k; void* v;
@@ -340,9 +341,9 @@ int b200fc_kv_append(const b200fc_kv_append_t* a, void* stream);
 
 /* out[r, h, :] = sum_j softmax_j(scale * q[r, h, :] . k_j) v_j over the cached tokens j of the row's sequence that are visible to its place p:
  * j <= p, and with window > 0 only the last `window` of them (j > p - window) and the first `sinks` tokens of the sequence (j < sinks).  Rows that see no
- * token, or none whose score is more than -inf, are zeros.  Scores, softmax and sums are fp32; probabilities are rounded to bf16 for the product with v.  H / Hkv query heads share a kv head
- * (any number).  max_rows, at least 1: no sequence has more rows (a sequence that has is left out, as above).  q and out bf16, 16-byte aligned with their strides; out overlaps
- * neither q nor the cache.  scale: any number below 2^127.
+ * token, or none whose score is more than -inf, are zeros.  Scores, softmax and sums are fp32; probabilities are rounded to bf16 for the product with v.
+ * H / Hkv query heads share a kv head (any number).  max_rows, at least 1: no sequence has more rows (a sequence that has is left out, as above).  q and out
+ * bf16, 16-byte aligned with their strides; out overlaps neither q nor the cache.  scale: any number below 2^127.
  * What lies behind a sequence's last token, or is invisible to all its rows, may be anything, NaN included.  k and v of visible tokens: any bf16, infinities
  * and NaN too; but the weights of v are divided by their sum only at the end, and may be 2^8 until then, so the result is finite only while the largest
  * finite |v| times the row's visible tokens is below 2^119.  8-bit cache: so too with |v| = 127 * v_scale, and k_scale and k_scale * |scale| below 2^121. */
